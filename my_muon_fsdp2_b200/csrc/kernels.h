@@ -317,4 +317,30 @@ int power_iteration_col_blocks(int m);
 void power_iteration(const void* W, bool w_f32, int m, int n, float* u, float* v, float* sigma, int iters,
                      float eps, float* work, float* col_part, cudaStream_t stream);
 
+// ----------------------------------------------------------------------------------------
+// Operators that take bf16, fp16 and fp32 values.
+enum class DType : int { BF16 = 0, F16 = 1, F32 = 2 };
+
+// Rotary positions of q [batch, seq, q_heads, head_dim] and k [batch, seq, k_heads, head_dim]
+// (k_heads may be 0) in one launch.  Strides are in elements, for batch, seq and head; the last
+// dimension is contiguous.  turns[rotary_dim / 2]: frequency of each pair in turns per position,
+// as 64-bit fixed point fractions of a turn.  positions: null (0..seq-1), or int64 / int32 values
+// at [b * pos_stride_b + t * pos_stride_t].  in_place: outputs are the inputs, and the part of
+// the head behind rotary_dim is not touched.
+struct RotaryArgs {
+  const void *q_in, *k_in;
+  void *q_out, *k_out;
+  int64_t q_in_s[3], k_in_s[3], q_out_s[3], k_out_s[3];
+  uint32_t batch, seq;
+  int q_heads, k_heads, head_dim, rotary_dim;
+  const uint64_t* turns;
+  const void* positions;
+  bool positions_32;
+  int64_t pos_stride_b, pos_stride_t;
+  float magnitude;  // factor on cos and sin
+  bool inverse, interleaved, in_place;
+  DType dtype;
+};
+void rotary(const RotaryArgs& args, cudaStream_t stream);
+
 }  // namespace mmf

@@ -34,6 +34,7 @@ SOURCES = [
     "model_kernels.cu",
     "attention.cu",
     "symm_comm.cu",
+    "rotary.cu",
     "noalloc.cu",
 ]
 
