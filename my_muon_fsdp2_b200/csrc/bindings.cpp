@@ -896,98 +896,6 @@ std::vector<Tensor> attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Ten
   return {dq, dk, dv};
 }
 
-mmf::DType dtype_of(const Tensor& t, const char* name) {
-  const auto d = t.scalar_type();
-  TORCH_CHECK(d == torch::kBFloat16 || d == torch::kFloat16 || d == torch::kFloat32, "mmf: ", name,
-              " must be bf16, fp16 or fp32");
-  return d == torch::kBFloat16 ? mmf::DType::BF16 : d == torch::kFloat16 ? mmf::DType::F16 : mmf::DType::F32;
-}
-
-// Rotary positions of q and k, [batch, seq, heads, head_dim] or [tokens, heads, head_dim]: the new
-// (contiguous) tensors, or q and k themselves.
-std::vector<Tensor> rotary(Tensor q, c10::optional<Tensor> k, c10::optional<Tensor> positions, Tensor turns,
-                           int64_t rotary_dim, bool interleaved, double magnitude, bool inverse, bool in_place) {
-  check_cuda(q, "q");
-  const c10::cuda::CUDAGuard guard(q.device());
-  const bool pair = k.has_value();
-  mmf::RotaryArgs a{};
-  a.dtype = dtype_of(q, "q");
-  const int64_t es = q.element_size(), nd = q.dim();
-  TORCH_CHECK(nd == 3 || nd == 4, "mmf: rotary takes [batch, seq, heads, head_dim] or [tokens, heads, head_dim]");
-  const int64_t B = nd == 4 ? q.size(0) : 1, T = q.size(nd - 3), D = q.size(nd - 1);
-  TORCH_CHECK(B * T <= 0x7fffffff, "mmf: rotary: too many tokens");
-  TORCH_CHECK(rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= D && D % 2 == 0 && D <= 256,
-              "mmf: rotary: head_dim and rotary_dim must be even, rotary_dim <= head_dim <= 256");
-  TORCH_CHECK(turns.device() == q.device() && turns.scalar_type() == torch::kInt64 && turns.is_contiguous() &&
-                  turns.numel() == rotary_dim / 2, "mmf: rotary: turns must be int64 [rotary_dim / 2] on q's device");
-  if (pair)
-    TORCH_CHECK(k->device() == q.device() && k->scalar_type() == q.scalar_type() && k->dim() == nd &&
-                    k->sizes().slice(0, nd - 2) == q.sizes().slice(0, nd - 2) && k->size(nd - 1) == D,
-                "mmf: rotary: q and k must agree in batch, seq, head_dim, dtype and device");
-  // strides for batch, seq and head (0 along dimensions of one element, whose stride is not used)
-  auto strides = [&](const Tensor& t, int64_t* s) {
-    s[0] = (nd == 4 && t.size(0) > 1) ? t.stride(0) : 0;
-    s[1] = t.size(nd - 3) > 1 ? t.stride(nd - 3) : 0;
-    s[2] = t.size(nd - 2) > 1 ? t.stride(nd - 2) : 0;
-  };
-  auto input = [&](Tensor t, int64_t* s) {
-    strides(t, s);
-    bool ok = t.numel() == 0 || t.stride(nd - 1) == 1;
-    if (interleaved)  // a pair is one access
-      ok = ok && reinterpret_cast<uintptr_t>(t.data_ptr()) % (2 * es) == 0 && s[0] % 2 == 0 && s[1] % 2 == 0 &&
-           s[2] % 2 == 0;
-    if (!ok) {
-      TORCH_CHECK(!in_place, "mmf: rotary: in place needs contiguous heads that start on a pair's boundary");
-      t = t.clone(at::MemoryFormat::Contiguous);
-      strides(t, s);
-    }
-    return t;
-  };
-  Tensor qi = input(q, a.q_in_s), ki, qo, ko;
-  if (pair) ki = input(*k, a.k_in_s);
-  if (in_place) {
-    qo = qi;
-    ko = ki;
-  } else {
-    qo = torch::empty(q.sizes(), q.options());
-    if (pair) ko = torch::empty(k->sizes(), k->options());
-  }
-  strides(qo, a.q_out_s);
-  if (pair) strides(ko, a.k_out_s);
-  a.q_in = qi.data_ptr();
-  a.q_out = qo.data_ptr();
-  a.k_in = pair ? ki.data_ptr() : nullptr;
-  a.k_out = pair ? ko.data_ptr() : nullptr;
-  a.batch = static_cast<uint32_t>(B);
-  a.seq = static_cast<uint32_t>(T);
-  a.q_heads = static_cast<int>(q.size(nd - 2));
-  a.k_heads = pair ? static_cast<int>(k->size(nd - 2)) : 0;
-  a.head_dim = static_cast<int>(D);
-  a.rotary_dim = static_cast<int>(rotary_dim);
-  a.turns = reinterpret_cast<const uint64_t*>(turns.data_ptr<int64_t>());
-  if (positions.has_value()) {
-    const Tensor& p = *positions;
-    const bool p32 = p.scalar_type() == torch::kInt32;
-    TORCH_CHECK(p.device() == q.device() && (p32 || p.scalar_type() == torch::kInt64),
-                "mmf: rotary: positions must be int64 or int32 on q's device");
-    const int64_t pd = p.dim();
-    TORCH_CHECK(pd >= 1 && pd <= nd - 2 && (p.size(pd - 1) == T || p.size(pd - 1) == 1) &&
-                    (pd == 1 || p.size(0) == B || p.size(0) == 1),
-                "mmf: rotary: positions must broadcast over batch and seq");
-    a.positions = p.data_ptr();
-    a.positions_32 = p32;
-    a.pos_stride_t = p.size(pd - 1) > 1 ? p.stride(pd - 1) : 0;
-    a.pos_stride_b = (pd == 2 && p.size(0) > 1) ? p.stride(0) : 0;
-  }
-  a.magnitude = static_cast<float>(magnitude);
-  a.inverse = inverse;
-  a.interleaved = interleaved;
-  a.in_place = in_place;
-  mmf::rotary(a, cur_stream());
-  if (pair) return {qo, ko};
-  return {qo};
-}
-
 int64_t device_error(int64_t device) {
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   return mmf::read_and_clear_device_error(static_cast<int>(device), cur_stream());
@@ -1004,6 +912,8 @@ bool device_checks() {
 }
 
 }  // namespace
+
+void register_lm_ops(pybind11::module_& m);  // bindings_lm.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels of my_muon_fsdp2_b200";
@@ -1051,7 +961,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_attention_fwd_variant", [](int64_t v) { mmf::set_attention_fwd_variant(static_cast<int>(v)); });
   m.def("set_gemm_variant", [](int64_t v) { mmf::set_gemm_variant(static_cast<int>(v)); });
   m.def("gemm_variant", []() { return static_cast<int64_t>(mmf::gemm_variant()); });
-  m.def("rotary", &rotary);
+  register_lm_ops(m);
   m.def("device_error", &device_error);
   m.def("launch_count", &launch_count);
   m.def("device_checks", &device_checks);

@@ -343,4 +343,37 @@ struct RotaryArgs {
 };
 void rotary(const RotaryArgs& args, cudaStream_t stream);
 
+// h = residual_scale * x + branch_scale * gate * norm_post(y) and, with pre_w, n = norm_pre(h),
+// over rows of `cols` values; norm is v / rms(v) * w, or with `layer` (v - mean) / std * w + b.
+// All rows are contiguous.  post_w, gate and pre_w may be null; a row r takes the gate's row
+// r / rows_per_gate.  stat_y and stat_h (fp32 [rows] for each present norm; with `layer` [rows, 2]:
+// 1 / std, mean) are written unless null.
+struct BlockNormArgs {
+  const void *x, *y, *post_w, *post_b, *gate, *pre_w, *pre_b;
+  void *h, *n;
+  float *stat_y, *stat_h;
+  int64_t rows, rows_per_gate;
+  int cols;
+  float eps, residual_scale, branch_scale;
+  bool layer;
+  DType dtype;
+};
+void block_norm_fwd(const BlockNormArgs& args, cudaStream_t stream);
+
+// Its backward: dx, dy and the gradients of the weights, biases and gate (null: not wanted).
+// dn and dh may each be null (zero).  parts: fp32 scratch of block_norm_bwd_parts(...) values.
+struct BlockNormBwdArgs {
+  const void *dh, *dn, *h, *y, *post_w, *post_b, *gate, *pre_w;
+  const float *stat_y, *stat_h;
+  void *dx, *dy, *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
+  float* parts;
+  int64_t rows, rows_per_gate;
+  int cols;
+  float residual_scale, branch_scale;
+  bool layer;
+  DType dtype;
+};
+int64_t block_norm_bwd_parts(const BlockNormBwdArgs& args);
+void block_norm_bwd(const BlockNormBwdArgs& args, cudaStream_t stream);
+
 }  // namespace mmf

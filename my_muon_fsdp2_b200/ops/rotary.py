@@ -12,7 +12,6 @@ from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._ext import ext
 
@@ -150,24 +149,6 @@ def _rotate_torch(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rot: Ro
     return r if R == x.shape[-1] else torch.cat((r, x[..., R:]), dim=-1)
 
 
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, rot, positions):
-        ctx.rot, ctx.pair = rot, k is not None
-        ctx.save_for_backward(positions)
-        out = ext().rotary(q, k, positions, rot._table(q.device), rot.rotary_dim, rot.interleaved, rot.magnitude,
-                           False, False)
-        return tuple(out) if ctx.pair else out[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk=None):
-        rot = ctx.rot
-        out = ext().rotary(dq, dk, ctx.saved_tensors[0], rot._table(dq.device), rot.rotary_dim, rot.interleaved,
-                           rot.magnitude, True, False)
-        return out[0], (out[1] if ctx.pair else None), None, None
-
-
 def _check(q, k, rot, positions, inplace) -> None:
     if not isinstance(rot, RotaryEmbedding):
         raise TypeError("apply_rotary: rotary must be a RotaryEmbedding")
@@ -219,8 +200,6 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotaryEmbed
         if inplace:
             out = [x.copy_(o) for x, o in zip((q, k), out)]
         return tuple(out) if k is not None else out[0]
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryFn.apply(q, k, rotary, positions)
     out = ext().rotary(q, k, positions, rotary._table(q.device), rotary.rotary_dim, rotary.interleaved,
-                       rotary.magnitude, False, inplace)
+                       rotary.magnitude, inplace)
     return tuple(out) if k is not None else out[0]

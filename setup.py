@@ -28,6 +28,7 @@ if os.environ.get("MMF_DEVICE_CHECKS", "0") == "1":
 
 SOURCES = [
     "bindings.cpp",
+    "bindings_lm.cpp",
     "tc_gemm.cu",
     "linear_gemm.cu",
     "optim_kernels.cu",
@@ -35,6 +36,8 @@ SOURCES = [
     "attention.cu",
     "symm_comm.cu",
     "rotary.cu",
+    "block_norm.cu",
+    "block_norm_bwd.cu",
     "noalloc.cu",
 ]
 
