@@ -306,9 +306,215 @@ std::vector<Tensor> block_norm(const Tensor& x, const Tensor& y, const OptTensor
   return BlockNormFn::apply(x, y, pw, pb, gate, nw, nb, rows_per_gate, layer, eps, residual_scale, branch_scale);
 }
 
+// ------------------------------------ distillation ----------------------------------------
+struct DistillConf {
+  double tau, alpha;
+  int64_t ignore_index;
+};
+
+// Checks the teacher's slots and the targets of `rows` rows and puts them into the arguments.
+mmf::DistillArgs distill_args(const Tensor& like, int64_t rows, int64_t vocab, const Tensor& ids, const Tensor& teacher,
+                              const OptTensor& targets, const DistillConf& c) {
+  check_cuda(like, "logits");
+  mmf::DistillArgs a{};
+  const auto it = ids.scalar_type();
+  TORCH_CHECK(ids.device() == like.device() && ids.dim() == 2 && ids.size(0) == rows && ids.is_contiguous() &&
+                  (it == torch::kInt64 || it == torch::kInt32),
+              "mmf: distill: ids must be contiguous int64 or int32 [rows, top] on the logits' device");
+  TORCH_CHECK(teacher.device() == like.device() && teacher.is_contiguous() && teacher.sizes() == ids.sizes(),
+              "mmf: distill: the teacher's logits must be contiguous, of the ids' shape, on the logits' device");
+  TORCH_CHECK(ids.size(1) >= 1 && ids.size(1) <= mmf::distill_max_top(), "mmf: distill: 1 to ", mmf::distill_max_top(),
+              " slots a row are supported");
+  a.dtype = dtype_of(like, "logits");
+  TORCH_CHECK(vocab >= 1 && vocab <= mmf::distill_max_vocab(a.dtype), "mmf: distill: a vocabulary of up to ",
+              mmf::distill_max_vocab(a.dtype), " values of this dtype is supported");
+  if (targets.has_value())
+    TORCH_CHECK(targets->device() == like.device() && targets->scalar_type() == torch::kInt64 &&
+                    targets->is_contiguous() && targets->numel() == rows,
+                "mmf: distill: targets must be contiguous int64 [rows] on the logits' device");
+  a.ids = ids.data_ptr();
+  a.ids_32 = it == torch::kInt32;
+  a.teacher = teacher.data_ptr();
+  a.teacher_dtype = dtype_of(teacher, "teacher logits");
+  a.targets = targets.has_value() ? targets->data_ptr<int64_t>() : nullptr;
+  a.rows = rows;
+  a.vocab = static_cast<int>(vocab);
+  a.top = static_cast<int>(ids.size(1));
+  a.tau = static_cast<float>(c.tau);
+  a.alpha = static_cast<float>(c.alpha);
+  a.ignore_index = c.ignore_index;
+  return a;
+}
+
+void put_logits(mmf::DistillArgs& a, const Tensor& logits) {
+  TORCH_CHECK(logits.dim() == 2 && (logits.numel() == 0 || logits.stride(1) == 1),
+              "mmf: distill: logits must be [rows, vocab] with unit column stride");
+  a.logits = logits.data_ptr();
+  a.ld = logits.size(0) > 1 ? logits.stride(0) : 0;
+}
+
+// A gradient of the logits whose rows lie as the logits' rows do against 16-byte boundaries (the
+// kernels move both through the same vectors): (the whole buffer, the rows in it).
+std::pair<Tensor, Tensor> grad_like(const Tensor& logits) {
+  const int64_t es = logits.element_size(), v = 16 / es, rows = logits.size(0), vocab = logits.size(1);
+  const int64_t ld = rows > 1 ? logits.stride(0) : 0;
+  const int64_t ld_g = vocab + ((ld - vocab) % v + v) % v;
+  const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16) / es;
+  Tensor flat = torch::empty({off + rows * ld_g}, logits.options());
+  return {flat, flat.as_strided({rows, vocab}, {ld_g, 1}, off)};
+}
+
+// int32 [2]: rows with a slot, rows with a target
+Tensor distill_count(const Tensor& like, int64_t vocab, const Tensor& ids, const Tensor& teacher,
+                     const OptTensor& targets, int64_t ignore_index) {
+  const c10::cuda::CUDAGuard guard(like.device());
+  const auto a = distill_args(like, ids.size(0), vocab, ids, teacher, targets, {1.0, 1.0, ignore_index});
+  Tensor counts = torch::empty({2}, like.options().dtype(torch::kInt32));
+  mmf::distill_count(a, counts.data_ptr<int>(), cur_stream());
+  return counts;
+}
+
+// Overwrites the logits [rows, vocab] with their gradient; the loss of each row goes to `loss`.
+void distill_rows_(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const OptTensor& targets, double tau,
+                   double alpha, int64_t ignore_index, const Tensor& counts, const Tensor& loss) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  auto a = distill_args(logits, logits.size(0), logits.size(1), ids, teacher, targets, {tau, alpha, ignore_index});
+  put_logits(a, logits);
+  TORCH_CHECK(counts.device() == logits.device() && counts.scalar_type() == torch::kInt32 && counts.numel() == 2,
+              "mmf: distill: counts must be int32 [2]");
+  TORCH_CHECK(loss.device() == logits.device() && loss.scalar_type() == torch::kFloat32 && loss.is_contiguous() &&
+                  loss.numel() == a.rows, "mmf: distill: loss must be contiguous fp32 [rows]");
+  a.grad = logits.data_ptr();
+  a.grad_ld = a.ld;
+  a.counts = counts.data_ptr<int>();
+  a.loss = loss.data_ptr<float>();
+  mmf::distill_rows(a, cur_stream());
+}
+
+Tensor distill_sum(const Tensor& loss) {
+  check_cuda(loss, "loss");
+  TORCH_CHECK(loss.scalar_type() == torch::kFloat32 && loss.is_contiguous(), "mmf: distill: loss must be contiguous fp32");
+  const c10::cuda::CUDAGuard guard(loss.device());
+  Tensor out = torch::empty({}, loss.options());
+  mmf::distill_sum(loss.data_ptr<float>(), loss.numel(), out.data_ptr<float>(), cur_stream());
+  return out;
+}
+
+// x *= s, s a one-element fp32 CUDA tensor read on the device; nothing is moved when it is 1
+void distill_scale_(const Tensor& x, const Tensor& s) {
+  check_cuda(x, "x");
+  TORCH_CHECK(x.is_contiguous() && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && s.device() == x.device() &&
+                  s.scalar_type() == torch::kFloat32 && s.numel() == 1,
+              "mmf: distill_scale_ takes a contiguous x on a 16-byte boundary and a one-element fp32 scale");
+  const c10::cuda::CUDAGuard guard(x.device());
+  mmf::distill_scale(x.data_ptr(), s.data_ptr<float>(), x.numel(), dtype_of(x, "x"), cur_stream());
+}
+
+// Whether the gradient is formed in the forward pass (one reading of the logits for both), to be
+// multiplied by the incoming gradient when that is not 1: where there is one such factor, for types
+// whose range does not need it beforehand.  fp16 gradients of a mean underflow without their loss
+// scale, and a factor for each row would cost a second pass as a rule: both form it in the backward
+// pass, from the logits and three kept values a row.
+bool grad_in_forward(const Tensor& logits, bool mean) { return mean && logits.scalar_type() != torch::kFloat16; }
+
+Tensor distill_forward(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const OptTensor& targets,
+                       const DistillConf& c, bool mean, const Tensor& grad, const Tensor& stats) {
+  auto a = distill_args(logits, logits.size(0), logits.size(1), ids, teacher, targets, c);
+  put_logits(a, logits);
+  if (grad.defined()) {
+    a.grad = grad.data_ptr();
+    a.grad_ld = grad.stride(0);
+  }
+  if (stats.defined()) a.stats = stats.data_ptr<float>();
+  Tensor counts;
+  if (mean) {
+    counts = distill_count(logits, a.vocab, ids, teacher, targets, c.ignore_index);
+    a.counts = counts.data_ptr<int>();
+  }
+  Tensor loss = torch::empty({a.rows}, logits.options().dtype(torch::kFloat32));
+  a.loss = loss.data_ptr<float>();
+  mmf::distill_rows(a, cur_stream());
+  return mean ? distill_sum(loss) : loss;
+}
+
+class DistillFn : public torch::autograd::Function<DistillFn> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& ids, const Tensor& teacher,
+                        const OptTensor& targets, double tau, double alpha, int64_t ignore_index, bool mean) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const DistillConf c{tau, alpha, ignore_index};
+    auto& d = ctx->saved_data;
+    if (grad_in_forward(logits, mean)) {
+      auto [flat, grad] = grad_like(logits);
+      d["flat"] = flat;
+      d["grad"] = grad;
+      return distill_forward(logits, ids, teacher, targets, c, mean, grad, Tensor());
+    }
+    Tensor stats = torch::empty({logits.size(0), 3}, logits.options().dtype(torch::kFloat32));
+    Tensor loss = distill_forward(logits, ids, teacher, targets, c, mean, Tensor(), stats);
+    ctx->save_for_backward({logits, ids, teacher, targets.value_or(Tensor()), stats});
+    d["tau"] = tau;
+    d["alpha"] = alpha;
+    d["ignore"] = ignore_index;
+    d["mean"] = mean;
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    refuse_second_order("distill");
+    auto& d = ctx->saved_data;
+    variable_list out(8);
+    Tensor up = g[0].to(torch::kFloat32).contiguous();
+    const c10::cuda::CUDAGuard guard(up.device());
+    if (ctx->get_saved_variables().empty()) {
+      TORCH_CHECK(d.count("grad"), "mmf: distill: this loss keeps its gradient for one backward pass; its graph cannot "
+                                   "be gone through a second time");
+      distill_scale_(d["flat"].toTensor(), up);
+      out[0] = d["grad"].toTensor();
+      d.clear();
+      return out;
+    }
+    const auto s = ctx->get_saved_variables();
+    const Tensor& logits = s[0];
+    const bool mean = d["mean"].toBool();
+    const int64_t ignore = d["ignore"].toInt();
+    const OptTensor targets = s[3].defined() ? OptTensor(s[3]) : OptTensor();
+    auto a = distill_args(logits, logits.size(0), logits.size(1), s[1], s[2], targets,
+                          {d["tau"].toDouble(), d["alpha"].toDouble(), ignore});
+    put_logits(a, logits);
+    Tensor counts;
+    if (mean) {
+      counts = distill_count(logits, a.vocab, s[1], s[2], targets, ignore);
+      a.counts = counts.data_ptr<int>();
+    }
+    out[0] = grad_like(logits).second;
+    a.grad = out[0].data_ptr();
+    a.grad_ld = out[0].stride(0);
+    a.stats = s[4].data_ptr<float>();
+    a.upstream = up.data_ptr<float>();
+    a.upstream_rows = !mean;
+    mmf::distill_grad(a, cur_stream());
+    return out;
+  }
+};
+
+Tensor distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const OptTensor& targets, double tau,
+               double alpha, int64_t ignore_index, bool mean) {
+  const OptTensor ol(logits);
+  if (wants_grad({&ol})) return DistillFn::apply(logits, ids, teacher, targets, tau, alpha, ignore_index, mean);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  return distill_forward(logits, ids, teacher, targets, {tau, alpha, ignore_index}, mean, Tensor(), Tensor());
+}
+
 }  // namespace
 
 void register_lm_ops(pybind11::module_& m) {
   m.def("rotary", &rotary);
   m.def("block_norm", &block_norm);
+  m.def("distill", &distill);
+  m.def("distill_count", &distill_count);
+  m.def("distill_rows_", &distill_rows_);
+  m.def("distill_sum", &distill_sum);
+  m.def("distill_scale_", &distill_scale_);
 }

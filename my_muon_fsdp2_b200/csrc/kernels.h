@@ -376,4 +376,39 @@ struct BlockNormBwdArgs {
 int64_t block_norm_bwd_parts(const BlockNormBwdArgs& args);
 void block_norm_bwd(const BlockNormBwdArgs& args, cudaStream_t stream);
 
+// Distillation from a teacher's top logits.  For each row of `logits` [rows, vocab] (row stride
+// `ld`), with the teacher's `top` slots (ids [rows, top], values [rows, top]; a slot with a
+// negative id or a value of -inf is empty) p = softmax(value / tau) over the row's slots and
+//   kd = tau^2 sum_j p_j (log p_j - log softmax(logits / tau)[id_j])      (0 without a slot)
+//   ce = -log softmax(logits)[target]                                     (0 when ignored)
+//   loss = alpha * kd * wk + (1 - alpha) * ce * wc
+// wk = wc = 1, or with `counts` (int32 [2]: rows with a slot, rows with a target) 1 / max(1, count).
+// Row r of `grad` must start as far from a 16-byte boundary as row r of `logits`.  An id or a target
+// outside the vocabulary is recorded in the device error word and left out.
+struct DistillArgs {
+  const void* logits;
+  void* grad;  // d loss / d logits (may be `logits` itself); null: the loss alone
+  int64_t ld, grad_ld;
+  const void *ids, *teacher;
+  const int64_t* targets;  // null: alpha is 1
+  const int* counts;
+  float* loss;    // [rows]
+  float* stats;   // [rows, 3] for distill_grad: the row's maximum, log2 of its sums at tau and at 1; null: not kept
+  const float* upstream;  // distill_grad: d result / d loss, one value or one for each row
+  int64_t rows;
+  int vocab, top;
+  float tau, alpha;
+  int64_t ignore_index;
+  bool ids_32, upstream_rows;
+  DType dtype, teacher_dtype;
+};
+int64_t distill_max_vocab(DType dtype);
+int distill_max_top();
+void distill_count(const DistillArgs& args, int* counts, cudaStream_t stream);
+void distill_rows(const DistillArgs& args, cudaStream_t stream);
+void distill_grad(const DistillArgs& args, cudaStream_t stream);
+void distill_sum(const float* loss, int64_t rows, float* out, cudaStream_t stream);
+// x *= *s (contiguous); returns after one read of *s when it is 1
+void distill_scale(void* x, const float* s, int64_t n, DType dtype, cudaStream_t stream);
+
 }  // namespace mmf

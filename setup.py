@@ -38,6 +38,7 @@ SOURCES = [
     "rotary.cu",
     "block_norm.cu",
     "block_norm_bwd.cu",
+    "distill.cu",
     "noalloc.cu",
 ]
 
