@@ -414,11 +414,12 @@ void distill_scale_(const Tensor& x, const Tensor& s) {
 // multiplied by the incoming gradient when that is not 1: where there is one such factor, for types
 // whose range does not need it beforehand.  fp16 gradients of a mean underflow without their loss
 // scale, and a factor for each row would cost a second pass as a rule: both form it in the backward
-// pass, from the logits and three kept values a row.
+// pass, from the logits and four kept values a row.
 bool grad_in_forward(const Tensor& logits, bool mean) { return mean && logits.scalar_type() != torch::kFloat16; }
 
 Tensor distill_forward(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const OptTensor& targets,
-                       const DistillConf& c, bool mean, const Tensor& grad, const Tensor& stats) {
+                       const DistillConf& c, bool mean, const Tensor& grad, const Tensor& stats,
+                       Tensor* counts_kept = nullptr) {
   auto a = distill_args(logits, logits.size(0), logits.size(1), ids, teacher, targets, c);
   put_logits(a, logits);
   if (grad.defined()) {
@@ -430,6 +431,7 @@ Tensor distill_forward(const Tensor& logits, const Tensor& ids, const Tensor& te
   if (mean) {
     counts = distill_count(logits, a.vocab, ids, teacher, targets, c.ignore_index);
     a.counts = counts.data_ptr<int>();
+    if (counts_kept) *counts_kept = counts;
   }
   Tensor loss = torch::empty({a.rows}, logits.options().dtype(torch::kFloat32));
   a.loss = loss.data_ptr<float>();
@@ -451,9 +453,10 @@ class DistillFn : public torch::autograd::Function<DistillFn> {
       d["grad"] = grad;
       return distill_forward(logits, ids, teacher, targets, c, mean, grad, Tensor());
     }
-    Tensor stats = torch::empty({logits.size(0), 3}, logits.options().dtype(torch::kFloat32));
-    Tensor loss = distill_forward(logits, ids, teacher, targets, c, mean, Tensor(), stats);
-    ctx->save_for_backward({logits, ids, teacher, targets.value_or(Tensor()), stats});
+    Tensor stats = torch::empty({logits.size(0), 4}, logits.options().dtype(torch::kFloat32));
+    Tensor counts;
+    Tensor loss = distill_forward(logits, ids, teacher, targets, c, mean, Tensor(), stats, &counts);
+    ctx->save_for_backward({logits, ids, teacher, targets.value_or(Tensor()), stats, counts});
     d["tau"] = tau;
     d["alpha"] = alpha;
     d["ignore"] = ignore_index;
@@ -478,16 +481,11 @@ class DistillFn : public torch::autograd::Function<DistillFn> {
     const auto s = ctx->get_saved_variables();
     const Tensor& logits = s[0];
     const bool mean = d["mean"].toBool();
-    const int64_t ignore = d["ignore"].toInt();
     const OptTensor targets = s[3].defined() ? OptTensor(s[3]) : OptTensor();
     auto a = distill_args(logits, logits.size(0), logits.size(1), s[1], s[2], targets,
-                          {d["tau"].toDouble(), d["alpha"].toDouble(), ignore});
+                          {d["tau"].toDouble(), d["alpha"].toDouble(), d["ignore"].toInt()});
     put_logits(a, logits);
-    Tensor counts;
-    if (mean) {
-      counts = distill_count(logits, a.vocab, s[1], s[2], targets, ignore);
-      a.counts = counts.data_ptr<int>();
-    }
+    if (mean) a.counts = s[5].data_ptr<int>();
     out[0] = grad_like(logits).second;
     a.grad = out[0].data_ptr();
     a.grad_ld = out[0].stride(0);

@@ -7,19 +7,28 @@
 // Bound by memory: the logits are read once and, with the gradient, written once.  A row is spread
 // over a cluster of blocks, each holding its slice in shared memory (a 128256 wide bf16 row has 250
 // KB, one block's shared memory 227): one asynchronous copy in, the maximum and the sums over the
-// slice, one exchange of (maximum, sums) through distributed shared memory, and the gradient
-// straight out of the slice.  Several blocks an SM overlap one another's copies and arithmetic.
+// slice, one exchange of (maximum, sums) between the blocks, and the gradient straight out of the
+// slice.  Slices of up to 32 KB and 256 threads let six blocks share an SM and overlap one another's
+// copies, exchanges and stores; what bounds it is how long a row stays in its block, not the arithmetic
+// (with the exponentials left out it is as slow).  Measured, 4096 x 128256 bf16, 64 slots, tau 2 with hard
+// targets: 414 us (2.1 GB, 78 % of the copy rate); slices of 64 KB 445 us; the exchange by a barrier of
+// the cluster, whose release waits for every store before it, and five blocks an SM 510 us; blocks that
+// stay for many rows, two an SM, with copies ahead and the exponentials kept in registers between the
+// two passes 500 us.
 //
-// The maximum is joined first within a thread, then sums are scaled to the common maximum as they
-// are joined, so nothing overflows.  exp(z - max) is exp2((z - max) log2 e): the difference is taken
-// before the product, which keeps its rounding relative to the distance from the maximum.
+// The arithmetic goes through packed fp32 instructions, the maximum of 16-bit types is taken without
+// widening them, and at tau = 2 the softmax at 1 comes from the one at tau as its square (one
+// exponential a value instead of two: 236 instead of 320 us at 2048 rows).
+//
+// Every exponential is 2^(c z - R), one fused multiply-add before it.  The reference R is the rounded
+// product c max(z) of a thread, later of the row, and is itself what sums are kept against: its
+// rounding cancels.  Sums are scaled by 2^(R - R') as they are joined, so nothing overflows.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
-#include <utility>
 
 #include "kernels.h"
 #include "tc_common.cuh"
@@ -31,12 +40,16 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// Which exponentials a launch needs: one (one of the two losses, or tau = 1), those at 1 as the squares
+// of those at tau = 2, or two of their own.
+enum Mode { ONE, SQUARE, TWO };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -44,27 +57,43 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float teacher_value(const DistillArgs& a, int64_t i) {
-  if (a.teacher_dtype == DType::F32) return static_cast<const float*>(a.teacher)[i];
-  if (a.teacher_dtype == DType::BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.teacher)[i]);
-  return __half2float(static_cast<const __half*>(a.teacher)[i]);
+// A slot as it lies in memory: loading several and looking at them later lets their latencies overlap.
+struct RawSlot {
+  uint2 id;
+  uint32_t value;
+};
+__device__ __forceinline__ RawSlot load_slot(const DistillArgs& a, int64_t i) {
+  RawSlot r{make_uint2(0u, 0u), 0u};
+  if (a.ids_32)
+    r.id.x = static_cast<const uint32_t*>(a.ids)[i];
+  else
+    r.id = static_cast<const uint2*>(a.ids)[i];
+  if (a.teacher_dtype == DType::F32)
+    r.value = static_cast<const uint32_t*>(a.teacher)[i];
+  else
+    r.value = static_cast<const uint16_t*>(a.teacher)[i];
+  return r;
 }
-__device__ __forceinline__ int64_t slot_id(const DistillArgs& a, int64_t i) {
-  return a.ids_32 ? static_cast<const int*>(a.ids)[i] : static_cast<const int64_t*>(a.ids)[i];
+// (id, value): -1 and -inf for an empty slot; an id behind the vocabulary is empty, and bad.
+__device__ __forceinline__ void look_at(const DistillArgs& a, const RawSlot& r, int& id, float& v, bool& bad) {
+  const int64_t wide = a.ids_32 ? static_cast<int64_t>(static_cast<int>(r.id.x))
+                                : static_cast<int64_t>(static_cast<uint64_t>(r.id.y) << 32 | r.id.x);
+  if (a.teacher_dtype == DType::F32)
+    v = __uint_as_float(r.value);
+  else if (a.teacher_dtype == DType::BF16)
+    v = __uint_as_float(r.value << 16);
+  else
+    v = __half2float(__ushort_as_half(static_cast<uint16_t>(r.value)));
+  bad |= wide >= a.vocab;
+  const bool empty = wide < 0 || wide >= a.vocab || v == -INFINITY;
+  id = empty ? -1 : static_cast<int>(wide);
+  if (empty) v = -INFINITY;
 }
-// The slot's id, or -1 for an empty slot; an id behind the vocabulary is empty and recorded.
-__device__ __forceinline__ int valid_id(const DistillArgs& a, int64_t i, int* err) {
-  const int64_t id = slot_id(a, i);
-  if (id >= a.vocab) {
-    atomicCAS(err, 0, ERR_BAD_ARGUMENT);
-    return -1;
-  }
-  return id < 0 ? -1 : static_cast<int>(id);
+__device__ __forceinline__ int64_t load_target(const DistillArgs& a, int64_t row) {
+  return a.targets ? a.targets[row] : a.ignore_index;
 }
-// The row's target, or -1 where it is ignored; one outside the vocabulary is ignored and recorded.
-__device__ __forceinline__ int valid_target(const DistillArgs& a, int64_t row, int* err) {
-  if (a.targets == nullptr) return -1;
-  const int64_t y = a.targets[row];
+// The target, or -1 where it is ignored; one outside the vocabulary is ignored and recorded.
+__device__ __forceinline__ int look_at(const DistillArgs& a, int64_t y, int* err) {
   if (y == a.ignore_index) return -1;
   if (y < 0 || y >= a.vocab) {
     atomicCAS(err, 0, ERR_BAD_ARGUMENT);
@@ -73,403 +102,506 @@ __device__ __forceinline__ int valid_target(const DistillArgs& a, int64_t row, i
   return static_cast<int>(y);
 }
 
-// max with the sums at tau (s) and at 1 (h), as joined over any two disjoint parts of a row
+// The largest of some logits, and the sums of their exponentials at the temperature of c_a (s) and, in
+// the modes that have them, at 1 (h), against the references of that maximum.
 struct Part {
   float m, s, h;
 };
-__device__ __forceinline__ Part join(const Part& a, const Part& b, float c_tau) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.h + b.h};  // nothing but -inf (or NaN, which the sums carry)
-  const float da = a.m - m, db = b.m - m;
-  return {m, a.s * ex2(da * c_tau) + b.s * ex2(db * c_tau), a.h * ex2(da * kLog2e) + b.h * ex2(db * kLog2e)};
+template <int MODE>
+struct Reference {
+  float a, b;
+  __device__ __forceinline__ Reference(float m, float c_a) {
+    if (m == -INFINITY) m = 0.f;  // nothing but -inf (or NaN, which the sums carry): every term is 0
+    a = __fmul_rn(m, c_a);
+    b = MODE == TWO ? __fmul_rn(m, kLog2e) : 2.f * a;
+  }
+};
+// Over groups of `W` lanes, the same bits in each of them.
+template <int MODE, int W>
+__device__ __forceinline__ Part warp_join(Part p, float c_a) {
+  float m = p.m;
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const Reference<MODE> from(p.m, c_a), to(m, c_a);
+  // without a finite logit of its own a part is 0 (or NaN) against any reference
+  p.s *= p.m == -INFINITY ? 1.f : ex2(from.a - to.a);
+  if (MODE != ONE) p.h *= p.m == -INFINITY ? 1.f : ex2(from.b - to.b);
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
+    if (MODE != ONE) p.h += __shfl_xor_sync(0xffffffffu, p.h, o);
+  }
+  p.m = m;
+  return p;
 }
 
-// Rows of one tensor start anywhere on the type's own boundary: a row is a head of up to 7 values, a
-// body of 16-byte vectors and a tail.
+__device__ __forceinline__ float2 exp2_2(float2 a) { return make_float2(ex2(a.x), ex2(a.y)); }
+// 16 bytes of a row as pairs
 template <typename T>
-struct RowSplit {
-  static constexpr int V = 16 / static_cast<int>(sizeof(T));
-  int head, vecs, tail;
-  __device__ RowSplit(const T* p, int vocab) {
-    head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T));
-    head = min(head, vocab);
-    vecs = (vocab - head) / V;
-    tail = vocab - head - vecs * V;
+struct Vec {
+  static constexpr int N = 16 / static_cast<int>(sizeof(T));
+  static __device__ __forceinline__ void pairs(const uint4& w, float2 (&p)[N / 2]) {
+    float v[N];
+    unpack<T, N>(w, v);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) p[e] = make_float2(v[2 * e], v[2 * e + 1]);
+  }
+  static __device__ __forceinline__ uint4 from_pairs(const float2 (&p)[N / 2]) {
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      v[2 * e] = p[e].x;
+      v[2 * e + 1] = p[e].y;
+    }
+    return pack<T, N>(v);
   }
 };
 
-// The teacher's distribution over a row's slots, in shared memory: p and id (-1: empty).
-struct TeacherRow {
-  float* p;
-  int* id;
+// The largest value of several vectors; NaN is left out (the sums carry it).
+template <typename T>
+struct MaxOf {
+  float m = -INFINITY;
+  __device__ __forceinline__ void put(const uint4& w) {
+    m = fmaxf(fmaxf(fmaxf(m, __uint_as_float(w.x)), __uint_as_float(w.y)),
+              fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  __device__ __forceinline__ float get() const { return m; }
 };
-__device__ __forceinline__ float block_max(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int i = 1; i < kWarps; ++i) v = fmaxf(v, red[i]);
-  return v;
-}
-__device__ __forceinline__ float block_add(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int i = 1; i < kWarps; ++i) v += red[i];
-  return v;
-}
-// Fills t; returns whether the row has a slot.  All threads of the block call it.
-__device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t row, const TeacherRow& t, float* red,
-                                            int* err) {
-  const float c = kLog2e / a.tau;
-  float best = -INFINITY;
-  int any = 0;
-  for (int j = threadIdx.x; j < a.top; j += kThreads) {
-    const int64_t i = row * a.top + j;
-    int id = valid_id(a, i, err);
-    const float v = id >= 0 ? teacher_value(a, i) : -INFINITY;
-    if (v == -INFINITY) id = -1;
+template <typename T2>
+struct MaxOfHalves {
+  T2 m;
+  static __device__ __forceinline__ T2 as(uint32_t w) { return *reinterpret_cast<const T2*>(&w); }
+  __device__ __forceinline__ void put(const uint4& w) {
+    m = __hmax2(m, __hmax2(__hmax2(as(w.x), as(w.y)), __hmax2(as(w.z), as(w.w))));
+  }
+};
+template <>
+struct MaxOf<__nv_bfloat16> : MaxOfHalves<__nv_bfloat162> {
+  __device__ __forceinline__ MaxOf() { m = as(0xff80ff80u); }  // -inf
+  __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <>
+struct MaxOf<__half> : MaxOfHalves<__half2> {
+  __device__ __forceinline__ MaxOf() { m = as(0xfc00fc00u); }
+  __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+
+// The positions of a row that a block has.  Rows start anywhere on the type's own boundary: a row is
+// a head of up to 7 values, a body of 16-byte vectors and a tail; a row's first block has the head, its
+// last the tail, and each `each` vectors (the last what is left).
+template <typename T>
+struct Share {
+  static constexpr int V = Vec<T>::N;
+  int first, vecs;  // the block's vectors: the position of the first, how many
+  int lo, hi;       // all its positions
+  int edges;        // how many of them are head and tail
+  int behind;       // where the row's tail starts
+  __device__ __forceinline__ Share(const T* row, int vocab, int each, int part, int parts) {
+    const int head = min(static_cast<int>(-reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T)), vocab);
+    const int all = (vocab - head) / V;
+    const int v0 = min(each * part, all);
+    vecs = min(each, all - v0);
+    first = head + v0 * V;
+    behind = head + all * V;
+    lo = part == 0 ? 0 : first;
+    hi = part == parts - 1 ? vocab : first + vecs * V;
+    edges = (hi - lo) - vecs * V;
+  }
+  __device__ __forceinline__ bool has(int v) const { return v >= lo && v < hi; }
+  // the i-th of the head's and the tail's positions
+  __device__ __forceinline__ int edge(int i) const { return i < first - lo ? lo + i : behind + i - (first - lo); }
+};
+
+// A row's slots in shared memory: p and id (-1: empty), `z` their logits where those are wanted, and the
+// numbers of the slots at this block's own positions.
+struct Slots {
+  float *p, *z;
+  int *id, *own;
+  __device__ __forceinline__ Slots(void* at, int top) {
+    const int room = (top + 3) & ~3;  // read four at a time
+    p = static_cast<float*>(at);
+    z = p + room;
+    id = reinterpret_cast<int*>(z + room);
+    own = id + room;
+  }
+};
+// Step 1, all threads: the teacher's ids and values, and (z not null) the logits there, into shared
+// memory.  The id and the value of a slot are loaded side by side: what a block waits for here are two
+// latencies at most, beside that of its slice.
+template <typename T>
+__device__ __forceinline__ void load_slots(const DistillArgs& a, int64_t row, const T* z, const Slots& t, int* err) {
+  const int room = (a.top + 3) & ~3;
+  bool bad = false;
+  for (int j = threadIdx.x; j < room; j += kThreads) {
+    int id = -1;
+    float v = -INFINITY;
+    if (j < a.top) look_at(a, load_slot(a, row * a.top + j), id, v, bad);
+    if (z && id >= 0) t.z[j] = to_f32(z[id]);
     t.id[j] = id;
     t.p[j] = v;
-    best = fmaxf(best, v);
-    any |= id >= 0;
   }
-  any = __syncthreads_or(any);
-  if (!any) return false;
-  best = block_max(best, red);
+  if (bad) atomicCAS(err, 0, ERR_BAD_ARGUMENT);
+}
+// Step 2, one warp: the values become p.  Returns (whether the row has a slot, how many are the block's
+// own).
+template <typename T>
+__device__ __forceinline__ int2 fill_slots(const DistillArgs& a, float c_tau, const Slots& t, const Share<T>& share) {
+  const int lane = threadIdx.x & 31;
+  float best = -INFINITY;
+  int any = 0, owned = 0;
+  for (int j0 = 0; j0 < a.top; j0 += 32) {
+    const int j = j0 + lane;
+    const int id = j < a.top ? t.id[j] : -1;
+    if (id >= 0) best = fmaxf(best, t.p[j]);
+    any |= id >= 0;
+    const bool own = id >= 0 && share.has(id);
+    const unsigned ballot = __ballot_sync(0xffffffffu, own);
+    if (own) t.own[owned + __popc(ballot & ((1u << lane) - 1u))] = j;
+    owned += __popc(ballot);
+  }
+  if (!__any_sync(0xffffffffu, any)) return make_int2(0, 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
   float s = 0.f;
-  for (int j = threadIdx.x; j < a.top; j += kThreads) s += t.id[j] >= 0 ? ex2((t.p[j] - best) * c) : 0.f;
-  const float inv = 1.f / block_add(s, red);
-  for (int j = threadIdx.x; j < a.top; j += kThreads) t.p[j] = t.id[j] >= 0 ? ex2((t.p[j] - best) * c) * inv : 0.f;
-  __syncthreads();
-  return true;
+  for (int j = lane; j < a.top; j += 32) {  // each lane its own slots: nothing to wait for
+    const float e = t.id[j] >= 0 ? ex2((t.p[j] - best) * c_tau) : 0.f;
+    t.p[j] = e;
+    s += e;
+  }
+  const float inv = __fdividef(1.f, warp_sum(s));
+  for (int j = lane; j < a.top; j += 32) t.p[j] *= inv;
+  __syncwarp();
+  return make_int2(1, owned);
 }
 
-// One row's softmaxes and its gradient.  dense(z) = k_a q_a(z) + k_b q_b(z), where a is the softmax
-// at `c_a` / log2 e and b, when both temperatures are wanted, the one at 1; the slots take
-// sub_p * p_j off, the target sub_y.
-struct RowGrad {
-  bool soft, hard;  // whether the row has a slot / a target that counts
-  float m, c_a, l_a, l_b, k_a, k_b, sub_p, sub_y;
+// What a launch has in common, formed on the host.
+struct Scales {
+  float c_tau;       // log2 e / tau
+  float c_a;         // the same, or log2 e where the soft loss has no weight
+  float soft, hard;  // alpha tau, 1 - alpha
+};
+Scales scales(const DistillArgs& a) {
+  const float c = static_cast<float>(1.4426950408889634 / a.tau);
+  return {c, a.alpha > 0.f ? c : kLog2e, a.alpha * a.tau, 1.f - a.alpha};
+}
 
-  __device__ __forceinline__ RowGrad(const DistillArgs& a, bool has_slot, bool has_target)
-      : soft(has_slot && a.alpha > 0.f), hard(has_target && a.alpha < 1.f), m(0.f), l_a(0.f), l_b(0.f) {
-    c_a = soft ? kLog2e / a.tau : kLog2e;
-    sub_p = soft ? a.alpha * a.tau * (a.counts ? 1.f / max(1, a.counts[0]) : 1.f) : 0.f;
-    sub_y = hard ? (1.f - a.alpha) * (a.counts ? 1.f / max(1, a.counts[1]) : 1.f) : 0.f;
-    k_a = sub_p;
-    k_b = sub_y;
-    if (!two(a)) k_a += k_b;
-  }
-  // whether the row needs exponentials at two temperatures
-  __device__ __forceinline__ bool two(const DistillArgs& a) const { return soft && hard && a.tau != 1.f; }
-  template <bool TWO>
-  __device__ __forceinline__ float dense(float z) const {
-    const float d = z - m;
-    float g = k_a * ex2(fmaf(d, c_a, -l_a));
-    if (TWO) g = fmaf(k_b, ex2(fmaf(d, kLog2e, -l_b)), g);
-    return g;
+// A row's coefficients: its gradient is k_a q_a + k_b q_b, with sub_p p_j off at the slots and sub_y
+// off at the target; q_a is the softmax at tau (at 1 where only the target counts), q_b the one at 1.
+struct Coefficients {
+  float k_a, k_b, sub_p, sub_y;
+  template <int MODE>
+  static __device__ __forceinline__ Coefficients of(const Scales& s, const int* counts, bool soft, bool hard, float up) {
+    Coefficients c;
+    c.sub_p = soft ? s.soft * up : 0.f;
+    c.sub_y = hard ? s.hard * up : 0.f;
+    if (counts) {
+      c.sub_p = __fdividef(c.sub_p, static_cast<float>(max(1, counts[0])));
+      c.sub_y = __fdividef(c.sub_y, static_cast<float>(max(1, counts[1])));
+    }
+    c.k_a = MODE == ONE ? c.sub_p + c.sub_y : c.sub_p;
+    c.k_b = c.sub_y;
+    return c;
   }
 };
 
-// Rewrites the gradient at this block's slots and target, where the dense part alone was stored.
-// get(v, z): whether position v of the row is this block's, and its logit.  The first slot of an id
-// answers for all slots of that id, and for the target when it is that id.
-template <typename T, bool TWO, typename Get>
-__device__ __forceinline__ void put_slots(const RowGrad& r, const TeacherRow& t, int top, int target, T* grad,
-                                          const Get& get) {
-  for (int j = threadIdx.x; j <= top; j += kThreads) {
-    const int id = j < top ? (r.soft ? t.id[j] : -1) : (r.hard ? target : -1);
-    float z;
-    if (id < 0 || !get(id, z)) continue;
-    bool first = true;
+// The gradient before the slots' and the target's own terms, from the row's joined part: the sums'
+// reciprocals are in the factors.
+template <int MODE>
+struct Dense {
+  float2 c, r_a, r_b, log2e, f_a, f_b;
+  __device__ __forceinline__ Dense(const Coefficients& k, float c_a, const Part& p) {
+    const Reference<MODE> r(p.m, c_a);
+    c = make_float2(c_a, c_a);
+    r_a = make_float2(-r.a, -r.a);
+    r_b = make_float2(-r.b, -r.b);
+    log2e = make_float2(kLog2e, kLog2e);
+    const float a = __fdividef(k.k_a, p.s), b = MODE == ONE ? 0.f : __fdividef(k.k_b, p.h);
+    f_a = make_float2(a, a);
+    f_b = make_float2(b, b);
+  }
+  __device__ __forceinline__ float2 operator()(float2 z) const {
+    const float2 e = exp2_2(ffma2(z, c, r_a));
+    if (MODE == ONE) return fmul2(e, f_a);
+    if (MODE == SQUARE) return fmul2(e, ffma2(e, f_b, f_a));
+    return ffma2(exp2_2(ffma2(z, log2e, r_b)), f_b, fmul2(e, f_a));
+  }
+  __device__ __forceinline__ float one(float z) const { return (*this)(make_float2(z, z)).x; }
+};
+
+// Rewrites the gradient at this block's `owned` slots and at its target, where the dense part alone was
+// stored.  A lane a slot; the first slot of an id answers for all slots of that id, and for the target
+// when it is that id.  get(v): the logit at the block's position v.
+template <typename T, int MODE, typename Get>
+__device__ __forceinline__ void put_slots(const Dense<MODE>& dense, const Coefficients& k, const Slots& t, int top,
+                                          int owned, int target, const Share<T>& share, T* grad, const Get& get) {
+  const bool has_target = target >= 0 && share.has(target);
+  for (int i = threadIdx.x; i < owned + has_target; i += kThreads) {
+    const int j = i < owned ? t.own[i] : top;  // the target comes behind the slots
+    const int id = i < owned ? t.id[j] : target;
     float p = 0.f;
-    if (r.soft) {
-      for (int i = 0; i < top; ++i) {
-        if (t.id[i] != id) continue;
-        if (i < j) {
-          first = false;
-          break;
+    bool earlier = false;
+    if (owned) {
+      for (int o = 0; o < top; o += 4) {  // what fills the last four is no id
+        const int4 other = *reinterpret_cast<const int4*>(t.id + o);
+        if (other.x == id || other.y == id || other.z == id || other.w == id) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (t.id[o + e] == id) {
+              p += t.p[o + e];
+              earlier |= o + e < j;
+            }
+          }
         }
-        p += t.p[i];
       }
     }
-    if (!first) continue;
-    float g = r.dense<TWO>(z) - r.sub_p * p;
-    if (r.hard && id == target) g -= r.sub_y;
+    if (earlier) continue;
+    float g = dense.one(get(id)) - k.sub_p * p;
+    if (id == target) g -= k.sub_y;
     grad[id] = from_f32<T>(g);
   }
 }
 
-// max and sums of a slice in shared memory (and of at most one more value of this thread)
-template <typename T, bool TWO>
+template <typename T, int MODE>
+__device__ __forceinline__ void store_dense(const Dense<MODE>& dense, const uint4* from, uint4* to, int n) {
+  constexpr int P = Vec<T>::N / 2;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    float2 p[P];
+    Vec<T>::pairs(from[i], p);
+#pragma unroll
+    for (int e = 0; e < P; ++e) p[e] = dense(p[e]);
+    to[i] = Vec<T>::from_pairs(p);
+  }
+}
+
+// Maximum and sums of a slice in shared memory, and of one more value of the first threads.
+template <typename T, int MODE>
 __device__ __forceinline__ Part slice_part(const uint4* slice, int n, bool has_edge, float edge, float c_a) {
-  constexpr int V = RowSplit<T>::V;
-  Part part{has_edge ? edge : -INFINITY, 0.f, 0.f};
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    float v[V];
-    unpack<T, V>(slice[i], v);
-#pragma unroll
-    for (int e = 0; e < V; ++e) part.m = fmaxf(part.m, v[e]);
-  }
-  const float m = part.m == -INFINITY ? 0.f : part.m;  // nothing but -inf: every term is 0
-  auto term = [&](float x) {
-    const float d = x - m;
-    part.s += ex2(d * c_a);
-    if (TWO) part.h += ex2(d * kLog2e);
+  constexpr int P = Vec<T>::N / 2;
+  MaxOf<T> most;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += kThreads) most.put(slice[i]);
+  Part part{most.get(), 0.f, 0.f};
+  if (has_edge) part.m = fmaxf(part.m, edge);
+  const Reference<MODE> r(part.m, c_a);
+  const float2 r_a = make_float2(-r.a, -r.a), r_b = make_float2(-r.b, -r.b), c = make_float2(c_a, c_a);
+  const float2 log2e = make_float2(kLog2e, kLog2e);
+  float2 s = make_float2(0.f, 0.f), h = s;
+  auto term = [&](float2 z) {
+    const float2 e = exp2_2(ffma2(z, c, r_a));
+    s = fadd2(s, e);
+    if (MODE == SQUARE) h = ffma2(e, e, h);
+    if (MODE == TWO) h = fadd2(h, exp2_2(ffma2(z, log2e, r_b)));
   };
-  if (has_edge) term(edge);
+  if (has_edge) term(make_float2(edge, -INFINITY));
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    float v[V];
-    unpack<T, V>(slice[i], v);
+    float2 p[P];
+    Vec<T>::pairs(slice[i], p);
 #pragma unroll
-    for (int e = 0; e < V; ++e) term(v[e]);
+    for (int e = 0; e < P; ++e) term(p[e]);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Part q;
-    q.m = __shfl_xor_sync(0xffffffffu, part.m, o);
-    q.s = __shfl_xor_sync(0xffffffffu, part.s, o);
-    q.h = __shfl_xor_sync(0xffffffffu, part.h, o);
-    part = join(part, q, c_a);
-  }
-  return part;
+  part.s = s.x + s.y;
+  part.h = h.x + h.y;
+  return warp_join<MODE, 32>(part, c_a);
 }
 
-template <typename T, bool TWO>
-__device__ __forceinline__ void store_dense(const RowGrad& r, const uint4* from, uint4* to, int n) {
-  constexpr int V = RowSplit<T>::V;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    float v[V];
-    unpack<T, V>(from[i], v);
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = r.dense<TWO>(v[e]);
-    to[i] = pack<T, V>(v);
-  }
+// 16 bytes to the same place in another block's shared memory, counted on that block's barrier.
+__device__ __forceinline__ void send(const void* to, uint64_t* bar, int block, float4 v) {
+  uint32_t remote, remote_bar;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(to)), "r"(block));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote_bar) : "r"(smem_u32(bar)), "r"(block));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(remote),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(remote_bar)
+               : "memory");
 }
 
-// One row a cluster.  Shared memory: the block's slice of the row, p and id of the slots.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_rows_kernel(const DistillArgs a, int* err) {
-  constexpr int V = RowSplit<T>::V;
+// One row a cluster.  Shared memory: the block's slice of the row, then the row's slots.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kThreads, 6) distill_rows_kernel(const DistillArgs a, const Scales sc, int each, int* err) {
+  constexpr int V = Vec<T>::N;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float red[kWarps];
   __shared__ Part warp_part[kWarps];
-  __shared__ Part block_part[kMaxCluster];  // every block's part, as each block of the cluster has it
-  __shared__ float edge[2 * V];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank()), blocks = static_cast<int>(cluster.num_blocks());
-  auto started = cluster.barrier_arrive();  // waited for before the first write to another block's memory
-  const int64_t row = blockIdx.x / blocks;
+  __shared__ float4 block_part[kMaxCluster];  // every block's part, as each block of the cluster has it
+  __shared__ __align__(8) uint64_t received;
+  __shared__ int2 row_slots;
+  __shared__ float target_z;
+  __shared__ float edge_value[2 * V];  // the head's and the tail's logits
+  // Parts travel as asynchronous stores that count their bytes on the receiver's barrier; every block
+  // of the cluster has to have that before the first is sent.
+  if (threadIdx.x == 0) {
+    mbar_init(&received, 1);
+    fence_mbar_init();
+    mbar_arrive_expect_tx(&received, gridDim.y * static_cast<uint32_t>(sizeof(float4)));
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int rank = static_cast<int>(blockIdx.y), blocks = static_cast<int>(gridDim.y);
+  const int64_t row = blockIdx.x;
   const T* z = static_cast<const T*>(a.logits) + row * a.ld;
-
-  const RowSplit<T> split(z, a.vocab);
-  const int v0 = static_cast<int>(static_cast<int64_t>(split.vecs) * rank / blocks);
-  const int n = static_cast<int>(static_cast<int64_t>(split.vecs) * (rank + 1) / blocks) - v0;
-  const int head = rank == 0 ? split.head : 0, tail = rank == blocks - 1 ? split.tail : 0;
-  const int behind = split.head + split.vecs * V;  // where the tail starts
+  const Share<T> share(z, a.vocab, each, rank, blocks);
+  const int n = share.vecs, tid = static_cast<int>(threadIdx.x), lane = tid & 31;
   uint4* slice = reinterpret_cast<uint4*>(smem);
-  TeacherRow t;
-  t.p = reinterpret_cast<float*>(slice + a.vocab / V / blocks + 1);
-  t.id = reinterpret_cast<int*>(t.p + a.top);
+  const Slots t(slice + each, a.top);
 
-  const uint4* body = reinterpret_cast<const uint4*>(z + split.head) + v0;
-  for (int i = threadIdx.x; i < n; i += kThreads)
+  const uint4* body = reinterpret_cast<const uint4*>(z + share.first);
+#pragma unroll 4
+  for (int i = tid; i < n; i += kThreads)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slice + i)), "l"(body + i) : "memory");
   asm volatile("cp.async.commit_group;" ::: "memory");
-  const int tid = static_cast<int>(threadIdx.x);
-  const bool has_edge = tid < head + tail;
-  const int edge_at = tid < head ? tid : behind + tid - head;
+  const bool has_edge = tid < share.edges;
+  const int edge_at = share.edge(tid);
   const float edge_z = has_edge ? to_f32(z[edge_at]) : 0.f;
-  if (has_edge) edge[tid] = edge_z;
 
-  const int target = valid_target(a, row, err);
-  RowGrad r(a, teacher_row(a, row, t, red, err), target >= 0);
-  const bool two = r.two(a), any = r.soft || r.hard;
-  // the first block has the loss: it gathers the logits of the slots and of the target before any
-  // block of the cluster can have written a gradient over them
-  float slot_z[kMaxTop / kThreads], target_z = 0.f;
-  if (rank == 0) {
-#pragma unroll
-    for (int k = 0; k < kMaxTop / kThreads; ++k) {
-      const int j = tid + k * kThreads;
-      slot_z[k] = r.soft && j < a.top && t.id[j] >= 0 ? to_f32(z[t.id[j]]) : 0.f;
-    }
-    if (r.hard) target_z = to_f32(z[target]);
-  }
-
+  // The first block has the loss: it gathers the logits of the slots and of the target before any
+  // block of the cluster can have written a gradient over them.
+  if (sc.soft > 0.f) load_slots(a, row, rank == 0 ? z : nullptr, t, err);
+  const int target = sc.hard > 0.f ? look_at(a, load_target(a, row), err) : -1;
+  if (rank == 0 && tid == 0 && target >= 0) target_z = to_f32(z[target]);
+  const float c_a = sc.c_a;
   asm volatile("cp.async.wait_all;" ::: "memory");
-  if (any) {
-    const Part p = two ? slice_part<T, true>(slice, n, has_edge, edge_z, r.c_a)
-                       : slice_part<T, false>(slice, n, has_edge, edge_z, r.c_a);
-    if ((tid & 31) == 0) warp_part[tid >> 5] = p;
+  const Part wp = slice_part<T, MODE>(slice, n, has_edge, edge_z, c_a);
+  if (lane == 0) warp_part[tid >> 5] = wp;
+  if (has_edge) edge_value[tid] = edge_z;
+  __syncthreads();  // also: the slice, the edges and the slots are there for the other threads
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (tid < 32) {
+    const Part p = warp_join<MODE, kWarps>(warp_part[lane % kWarps], c_a);
+    if (lane < blocks) send(&block_part[rank], &received, lane, make_float4(p.m, p.s, p.h, 0.f));
+  } else if (tid < 64) {
+    const int2 has = sc.soft > 0.f ? fill_slots(a, sc.c_tau, t, share) : make_int2(0, 0);
+    if (lane == 0) row_slots = has;
   }
-  __syncthreads();  // also: slices and edges are there for the other threads
-  if (any) {
-    Part p = warp_part[0];
-    for (int w = 1; w < kWarps; ++w) p = join(p, warp_part[w], r.c_a);
-    cluster.barrier_wait(std::move(started));
-    if (tid < blocks) *cluster.map_shared_rank(&block_part[rank], tid) = p;
-    cluster.sync();
-    p = block_part[0];
-    for (int b = 1; b < blocks; ++b) p = join(p, block_part[b], r.c_a);
-    r.m = p.m;
-    r.l_a = log2f(p.s);
-    r.l_b = two ? log2f(p.h) : r.l_a;
-  } else {
-    cluster.barrier_wait(std::move(started));
-  }
+  __syncthreads();  // row_slots
+  mbar_wait(&received, 0, err, ERR_PEER_FLAG_TIMEOUT, MMF_WAIT_TIMEOUT_NS, false);
+  const float4 part = lane % kMaxCluster < blocks ? block_part[lane % kMaxCluster] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  const Part p = warp_join<MODE, kMaxCluster>(Part{part.x, part.y, part.z}, c_a);
+  const bool soft = row_slots.x, hard = target >= 0;
+  const Coefficients k = Coefficients::of<MODE>(sc, a.counts, soft, hard, 1.f);
 
-  if (rank == 0) {
+  auto put_loss = [&]() {
+    if (rank != 0 || tid >= 32) return;
+    const Reference<MODE> r(p.m, c_a);
+    const float l_a = log2f(p.s);
     float kd = 0.f;  // sum p_j (log2 p_j - log2 q_tau(id_j))
-    if (r.soft) {
-#pragma unroll
-      for (int k = 0; k < kMaxTop / kThreads; ++k) {
-        const int j = tid + k * kThreads;
-        if (j < a.top && t.id[j] >= 0 && t.p[j] > 0.f)
-          kd = fmaf(t.p[j], log2f(t.p[j]) - fmaf(slot_z[k] - r.m, r.c_a, -r.l_a), kd);
-      }
-      kd = block_add(kd, red);
+    if (soft) {
+      for (int j = lane; j < a.top; j += 32)
+        if (t.id[j] >= 0 && t.p[j] > 0.f) kd = fmaf(t.p[j], log2f(t.p[j]) - (fmaf(t.z[j], c_a, -r.a) - l_a), kd);
+      kd = warp_sum(kd);
     }
-    if (tid == 0) {
-      const float ce = r.hard ? fmaf(r.l_b, kLn2, r.m - target_z) : 0.f;
+    if (lane == 0) {
+      const float ce = kLn2 * (MODE == ONE ? l_a - fmaf(target_z, c_a, -r.a) : log2f(p.h) - fmaf(target_z, kLog2e, -r.b));
       // sub_p = alpha tau / count; the loss has another tau
-      a.loss[row] = r.sub_p * a.tau * kLn2 * kd + r.sub_y * ce;
-      if (a.stats) {
-        a.stats[3 * row] = r.m;
-        a.stats[3 * row + 1] = r.l_a;
-        a.stats[3 * row + 2] = r.l_b;
-      }
+      a.loss[row] = (soft ? k.sub_p * a.tau * kLn2 * kd : 0.f) + (hard ? k.sub_y * ce : 0.f);
+      if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(p.m, p.s, p.h, soft ? 1.f : 0.f);
     }
-  }
-  if (a.grad == nullptr) return;
+  };
+  if (a.grad == nullptr) return put_loss();
 
   T* grad = static_cast<T*>(a.grad) + row * a.grad_ld;
-  uint4* to = reinterpret_cast<uint4*>(grad + split.head) + v0;
-  if (!any) {
+  uint4* to = reinterpret_cast<uint4*>(grad + share.first);
+  if (!soft && !hard) {  // takes no part, whatever its logits are
     for (int i = tid; i < n; i += kThreads) to[i] = make_uint4(0u, 0u, 0u, 0u);
     if (has_edge) grad[edge_at] = from_f32<T>(0.f);
-    return;
+    return put_loss();
   }
-  // position v of the row, if this block has it
-  auto get = [&](int v, float& x) {
-    if (v < split.head || v >= behind) {
-      if (rank != (v < split.head ? 0 : blocks - 1)) return false;
-      x = edge[v < split.head ? v : head + v - behind];
-      return true;
-    }
-    const int i = (v - split.head) / V - v0;
-    if (i < 0 || i >= n) return false;
-    x = to_f32(reinterpret_cast<const T*>(slice + i)[(v - split.head) % V]);
-    return true;
-  };
-  auto write = [&](auto mode) {
-    constexpr bool TWO = decltype(mode)::value;
-    store_dense<T, TWO>(r, slice, to, n);
-    if (has_edge) grad[edge_at] = from_f32<T>(r.dense<TWO>(edge_z));
-    __syncthreads();  // the slots' rewrites come after the dense stores
-    put_slots<T, TWO>(r, t, a.top, target, grad, get);
-  };
-  if (two)
-    write(std::true_type());
-  else
-    write(std::false_type());
+  const Dense<MODE> dense(k, c_a, p);
+  store_dense<T, MODE>(dense, slice, to, n);
+  if (has_edge) grad[edge_at] = from_f32<T>(dense.one(edge_z));
+  __syncthreads();  // the slots' rewrites come after the dense stores
+  put_slots<T, MODE>(dense, k, t, a.top, row_slots.y, target, share, grad, [&](int v) {
+    if (v < share.first) return edge_value[v - share.lo];
+    const int at = v - share.first;
+    return at < n * V ? to_f32(reinterpret_cast<const T*>(slice)[at])
+                      : edge_value[share.first - share.lo + v - share.behind];
+  });
+  put_loss();
 }
 
 // The gradient alone, from the statistics of an earlier pass and the incoming gradient: blocks of
-// `segment` vectors of a row, straight from and to global memory.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_grad_kernel(const DistillArgs a, int segments, int segment,
-                                                                int* err) {
-  constexpr int V = RowSplit<T>::V;
+// `kSegment` vectors of a row, straight from and to global memory.
+constexpr int kSegment = kThreads * 8;
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kThreads) distill_grad_kernel(const DistillArgs a, const Scales sc, int* err) {
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float red[kWarps];
-  const int64_t row = blockIdx.x / segments;
-  const int seg = static_cast<int>(blockIdx.x - row * segments);
+  const int64_t row = blockIdx.x;
   const T* z = static_cast<const T*>(a.logits) + row * a.ld;
   T* grad = static_cast<T*>(a.grad) + row * a.grad_ld;
-  const RowSplit<T> split(z, a.vocab);
-  const int v0 = min(seg * segment, split.vecs), n = min(segment, split.vecs - v0);
-  const int behind = split.head + split.vecs * V;
-  const int head = seg == 0 ? split.head : 0, tail = seg == segments - 1 ? split.tail : 0;
+  const Share<T> share(z, a.vocab, kSegment, static_cast<int>(blockIdx.y), static_cast<int>(gridDim.y));
   const int tid = static_cast<int>(threadIdx.x);
-  const bool has_edge = tid < head + tail;
-  const int edge_at = tid < head ? tid : behind + tid - head;
-  const uint4* from = reinterpret_cast<const uint4*>(z + split.head) + v0;
-  uint4* to = reinterpret_cast<uint4*>(grad + split.head) + v0;
-
-  TeacherRow t;
-  t.p = reinterpret_cast<float*>(smem);
-  t.id = reinterpret_cast<int*>(t.p + a.top);
-  const int target = valid_target(a, row, err);
-  RowGrad r(a, teacher_row(a, row, t, red, err), target >= 0);
-  const bool two = r.two(a);
-  if (!r.soft && !r.hard) {
-    for (int i = tid; i < n; i += kThreads) to[i] = make_uint4(0u, 0u, 0u, 0u);
+  const bool has_edge = tid < share.edges;
+  const int edge_at = share.edge(tid);
+  const uint4* from = reinterpret_cast<const uint4*>(z + share.first);
+  uint4* to = reinterpret_cast<uint4*>(grad + share.first);
+  const Slots t(smem, a.top);
+  const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
+  const bool soft = st.w != 0.f;
+  const int target = sc.hard > 0.f ? look_at(a, load_target(a, row), err) : -1;
+  const bool hard = target >= 0;
+  if (!soft && !hard) {
+    for (int i = tid; i < share.vecs; i += kThreads) to[i] = make_uint4(0u, 0u, 0u, 0u);
     if (has_edge) grad[edge_at] = from_f32<T>(0.f);
     return;
   }
   const float up = a.upstream[a.upstream_rows ? row : 0];
-  r.k_a *= up;
-  r.k_b *= up;
-  r.sub_p *= up;
-  r.sub_y *= up;
-  r.m = a.stats[3 * row];
-  r.l_a = a.stats[3 * row + 1];
-  r.l_b = a.stats[3 * row + 2];
-  auto get = [&](int v, float& x) {
-    if (v < split.head || v >= behind) {
-      if (seg != (v < split.head ? 0 : segments - 1)) return false;
-    } else {
-      const int i = (v - split.head) / V - v0;
-      if (i < 0 || i >= n) return false;
-    }
-    x = to_f32(z[v]);
-    return true;
-  };
-  auto write = [&](auto mode) {
-    constexpr bool TWO = decltype(mode)::value;
-    store_dense<T, TWO>(r, from, to, n);
-    if (has_edge) grad[edge_at] = from_f32<T>(r.dense<TWO>(to_f32(z[edge_at])));
-    __syncthreads();
-    put_slots<T, TWO>(r, t, a.top, target, grad, get);
-  };
-  if (two)
-    write(std::true_type());
-  else
-    write(std::false_type());
+  const Coefficients k = Coefficients::of<MODE>(sc, a.counts, soft, hard, up);
+  const Dense<MODE> dense(k, sc.c_a, Part{st.x, st.y, st.z});
+  __shared__ int row_owned;
+  if (soft) load_slots<T>(a, row, nullptr, t, err);
+  __syncthreads();
+  if (tid < 32) {
+    const int owned = soft ? fill_slots(a, sc.c_tau, t, share).y : 0;
+    if (tid == 0) row_owned = owned;
+  }
+  store_dense<T, MODE>(dense, from, to, share.vecs);
+  if (has_edge) grad[edge_at] = from_f32<T>(dense.one(to_f32(z[edge_at])));
+  __syncthreads();  // the slots are there; their rewrites come after the dense stores
+  put_slots<T, MODE>(dense, k, t, a.top, row_owned, target, share, grad, [&](int v) { return to_f32(z[v]); });
 }
 
-// counts[0]: rows with a slot, counts[1]: rows with a target.  One block: a thread mostly reads its
-// rows' first slot alone.
-__global__ void __launch_bounds__(1024) distill_count_kernel(const DistillArgs a, int* counts, int* err) {
-  int slots = 0, targets = 0;
-  for (int64_t row = threadIdx.x; row < a.rows; row += blockDim.x) {
-    for (int j = 0; j < a.top; ++j) {
-      const int64_t i = row * a.top + j;
-      if (valid_id(a, i, err) >= 0 && !(teacher_value(a, i) == -INFINITY)) {
-        ++slots;
-        break;
-      }
-    }
-    targets += valid_target(a, row, err) >= 0;
-  }
+// counts[0]: rows with a slot, counts[1]: rows with a target.  One cluster: a lane looks at its row's
+// first slot, and the warp together at the rows where that one is empty.
+__global__ void __cluster_dims__(kMaxCluster, 1, 1) __launch_bounds__(1024)
+    distill_count_kernel(const DistillArgs a, int* counts, int* err) {
   __shared__ int s[2];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), lane = threadIdx.x & 31;
   if (threadIdx.x < 2) s[threadIdx.x] = 0;
-  __syncthreads();
+  cluster.sync();
+  int slots = 0, targets = 0;
+  bool bad = false;
+  auto filled = [&](int64_t row, int j) {
+    int id;
+    float v;
+    look_at(a, load_slot(a, row * a.top + j), id, v, bad);
+    return id >= 0;
+  };
+  for (int64_t base = (rank * 32 + (threadIdx.x >> 5)) * 32; base < a.rows; base += kMaxCluster * 1024) {
+    const int64_t mine = base + lane;
+    const bool live = mine < a.rows;
+    const int64_t y = live ? load_target(a, mine) : a.ignore_index;
+    const bool first = live && filled(mine, 0);
+    targets += look_at(a, y, err) >= 0;
+    slots += first;
+    for (unsigned rest = __ballot_sync(0xffffffffu, live && !first); rest; rest &= rest - 1) {
+      const int64_t row = base + __ffs(static_cast<int>(rest)) - 1;
+      bool any = false;
+#pragma unroll 2
+      for (int j = 1 + lane; j < a.top; j += 32) any |= filled(row, j);
+      any = __any_sync(0xffffffffu, any);
+      slots += any && lane == 0;
+    }
+  }
+  if (bad) atomicCAS(err, 0, ERR_BAD_ARGUMENT);
   slots = __reduce_add_sync(0xffffffffu, slots);
   targets = __reduce_add_sync(0xffffffffu, targets);
-  if ((threadIdx.x & 31) == 0) {  // whole numbers: the order does not matter
-    atomicAdd(&s[0], slots);
-    atomicAdd(&s[1], targets);
+  if (lane == 0) {  // whole numbers: the order does not matter
+    atomicAdd(cluster.map_shared_rank(&s[0], 0), slots);
+    atomicAdd(cluster.map_shared_rank(&s[1], 0), targets);
   }
-  __syncthreads();
-  if (threadIdx.x < 2) counts[threadIdx.x] = s[threadIdx.x];
+  cluster.sync();
+  if (rank == 0 && threadIdx.x < 2) counts[threadIdx.x] = s[threadIdx.x];
 }
 
 __global__ void __launch_bounds__(512) distill_sum_kernel(const float* loss, int64_t rows, float* out) {
@@ -524,9 +656,24 @@ void typed(DType d, const Go& go) {
     go(float());
 }
 
-constexpr int kSliceGoal = 64 << 10;  // bytes: three blocks an SM
+// Calls go(type, mode) with both as compile-time values.
+template <typename Go>
+void typed_mode(const DistillArgs& a, const Go& go) {
+  const bool both = a.alpha > 0.f && a.alpha < 1.f && a.targets && a.tau != 1.f;
+  typed(a.dtype, [&](auto t) {
+    if (!both)
+      go(t, std::integral_constant<int, ONE>());
+    else if (a.tau == 2.f)
+      go(t, std::integral_constant<int, SQUARE>());
+    else
+      go(t, std::integral_constant<int, TWO>());
+  });
+}
+
+constexpr int kSliceGoal = 32 << 10;  // bytes: six blocks an SM
 constexpr int kSliceMost = 200 << 10;
 constexpr int kSliceLeast = 8 << 10;
+int slot_bytes(int top) { return ((top + 3) & ~3) * 16; }
 
 }  // namespace
 
@@ -534,7 +681,7 @@ int64_t distill_max_vocab(DType dtype) { return kSliceMost / (dtype == DType::F3
 int distill_max_top() { return kMaxTop; }
 
 void distill_count(const DistillArgs& a, int* counts, cudaStream_t stream) {
-  distill_count_kernel<<<1, 1024, 0, stream>>>(a, counts, error_word());
+  distill_count_kernel<<<kMaxCluster, 1024, 0, stream>>>(a, counts, error_word());
   check("distill_count");
 }
 
@@ -542,32 +689,34 @@ void distill_rows(const DistillArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return;
   if (a.top < 1 || a.top > kMaxTop || a.vocab < 1 || a.vocab > distill_max_vocab(a.dtype))
     throw std::runtime_error("mmf: distill: vocabulary or number of slots out of range");
-  typed(a.dtype, [&](auto tag) {
+  typed_mode(a, [&](auto tag, auto mode) {
     using T = decltype(tag);
     const int64_t bytes = static_cast<int64_t>(a.vocab) * sizeof(T);
-    // blocks a row: slices that fit three to an SM; with few rows more, down to 8 KB each, so that
+    // blocks a row: slices that fit six to an SM; with few rows more, down to 8 KB each, so that
     // every SM has one
     int blocks = 1;
     while (blocks < kMaxCluster && bytes / blocks > kSliceGoal) blocks *= 2;
     while (blocks < kMaxCluster && a.rows * blocks < 148 && bytes / blocks > kSliceLeast) blocks *= 2;
-    if (a.rows * blocks > 0x7fffffff) throw std::runtime_error("mmf: distill: too many rows");
-    constexpr int V = 16 / static_cast<int>(sizeof(T));
-    const int smem = (a.vocab / V / blocks + 1) * 16 + a.top * 8;
-    auto kernel = distill_rows_kernel<T>;
+    if (a.rows > 0x7fffffff) throw std::runtime_error("mmf: distill: too many rows");
+    const int each = (a.vocab / Vec<T>::N + blocks - 1) / blocks;
+    const int smem = each * 16 + slot_bytes(a.top);
+    auto kernel = distill_rows_kernel<T, decltype(mode)::value>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) throw std::runtime_error(std::string("mmf: distill: ") + cudaGetErrorString(e));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(a.rows * blocks));
+    cfg.gridDim = dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(blocks));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(blocks);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    attr.val.clusterDim.x = attr.val.clusterDim.z = 1;
+    attr.val.clusterDim.y = static_cast<unsigned>(blocks);
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, a, error_word());
+    cudaLaunchKernelEx(&cfg, kernel, a, scales(a), each, error_word());
   });
   check("distill_rows");
 }
@@ -575,14 +724,13 @@ void distill_rows(const DistillArgs& a, cudaStream_t stream) {
 void distill_grad(const DistillArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return;
   if (a.top < 1 || a.top > kMaxTop) throw std::runtime_error("mmf: distill: number of slots out of range");
-  typed(a.dtype, [&](auto tag) {
+  typed_mode(a, [&](auto tag, auto mode) {
     using T = decltype(tag);
-    constexpr int V = 16 / static_cast<int>(sizeof(T));
-    const int segment = kThreads * 4;  // vectors
-    const int segments = std::max(1, (a.vocab / V + segment - 1) / segment);
-    if (a.rows * segments > 0x7fffffff) throw std::runtime_error("mmf: distill: too many rows");
-    distill_grad_kernel<T><<<static_cast<unsigned>(a.rows * segments), kThreads, a.top * 8, stream>>>(
-        a, segments, segment, error_word());
+    const int segments = std::max(1, (a.vocab / Vec<T>::N + kSegment - 1) / kSegment);
+    if (a.rows > 0x7fffffff || segments > 65535) throw std::runtime_error("mmf: distill: too many rows");
+    distill_grad_kernel<T, decltype(mode)::value>
+        <<<dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(segments)), kThreads, slot_bytes(a.top), stream>>>(
+            a, scales(a), error_word());
   });
   check("distill_grad");
 }

@@ -393,7 +393,7 @@ struct DistillArgs {
   const int64_t* targets;  // null: alpha is 1
   const int* counts;
   float* loss;    // [rows]
-  float* stats;   // [rows, 3] for distill_grad: the row's maximum, log2 of its sums at tau and at 1; null: not kept
+  float* stats;   // [rows, 4] for distill_grad: the row's maximum, its two sums, whether it has a slot; or null
   const float* upstream;  // distill_grad: d result / d loss, one value or one for each row
   int64_t rows;
   int vocab, top;
