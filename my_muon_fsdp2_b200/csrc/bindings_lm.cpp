@@ -228,9 +228,9 @@ class BlockNormFn : public torch::autograd::Function<BlockNormFn> {
     Tensor stat_y, stat_h;
     auto out = block_norm_raw(x, y, pw, pb, gate, nw, nb, {rows_per_gate, layer, eps, residual_scale, branch_scale},
                               &stat_y, &stat_h);
-    // y only comes back through its norm or the gate, h only through its norm
-    const bool keep_y = pw.has_value() || gate.has_value();
-    ctx->save_for_backward({keep_y ? y : Tensor(), nw.has_value() ? out[0] : Tensor(), pw.value_or(Tensor()),
+    // the backward forms h again from x and y for its norm; y comes back through its own norm and the gate
+    const bool keep_y = pw.has_value() || gate.has_value() || nw.has_value();
+    ctx->save_for_backward({keep_y ? y : Tensor(), nw.has_value() ? x : Tensor(), pw.value_or(Tensor()),
                             pb.value_or(Tensor()), gate.value_or(Tensor()), nw.value_or(Tensor()), stat_y, stat_h});
     auto& d = ctx->saved_data;
     d["rows_per_gate"] = rows_per_gate;
@@ -247,7 +247,7 @@ class BlockNormFn : public torch::autograd::Function<BlockNormFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     refuse_second_order("block_norm");
     auto saved = ctx->get_saved_variables();
-    const Tensor &y = saved[0], &h = saved[1], &pw = saved[2], &pb = saved[3], &gate = saved[4], &nw = saved[5];
+    const Tensor &y = saved[0], &x = saved[1], &pw = saved[2], &pb = saved[3], &gate = saved[4], &nw = saved[5];
     auto& d = ctx->saved_data;
     const int64_t need = d["need"].toInt();
     variable_list out(12);
@@ -274,7 +274,7 @@ class BlockNormFn : public torch::autograd::Function<BlockNormFn> {
     };
     a.dh = p(dh);
     a.dn = p(dn);
-    a.h = p(h);
+    a.x = p(x);
     a.y = p(y);
     a.post_w = p(pw);
     a.post_b = p(pb);

@@ -5,6 +5,7 @@
 #include <stdexcept>
 
 #include "kernels.h"
+#include "tc_common.cuh"
 #include "typed_io.cuh"
 
 namespace mmf {
@@ -15,7 +16,7 @@ namespace {
 // block takes part in every reduction.
 struct RowGroup {
   int tpr, row, lane, warp0, warps;
-  float* red;  // [2][3 * 32], used in turn so that one barrier a reduction is enough
+  float* red;  // [2][2][32], used in turn so that one barrier a reduction is enough; 16-byte aligned
   int turn = 0;
   __device__ RowGroup(int tpr_, float* red_) : tpr(tpr_), red(red_) {
     row = threadIdx.x / tpr;
@@ -31,7 +32,7 @@ struct RowGroup {
       if (b) *b += __shfl_xor_sync(0xffffffffu, *b, o);
     }
     if (warps == 1) return;
-    float* r = red + 96 * turn;
+    float* r = red + 64 * turn;
     turn ^= 1;
     const int w = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) {
@@ -39,39 +40,19 @@ struct RowGroup {
       if (b) r[32 + w] = *b;
     }
     __syncthreads();
-    a = 0.f;
-    if (b) *b = 0.f;
-    for (int i = 0; i < warps; ++i) {
-      a += r[warp0 + i];
-      if (b) *b += r[32 + warp0 + i];
-    }
+    a = over_warps(r + warp0);
+    if (b) *b = over_warps(r + 32 + warp0);
   }
-  // Joins (count, mean, sum of squared distances from the mean) over the row's threads.
-  __device__ __forceinline__ void join(float& n, float& mean, float& m2) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      merge(n, mean, m2, __shfl_xor_sync(0xffffffffu, n, o), __shfl_xor_sync(0xffffffffu, mean, o),
-            __shfl_xor_sync(0xffffffffu, m2, o));
-    if (warps == 1) return;
-    float* r = red + 96 * turn;
-    turn ^= 1;
-    const int w = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
-      r[w] = n;
-      r[32 + w] = mean;
-      r[64 + w] = m2;
+
+ private:
+  __device__ __forceinline__ float over_warps(const float* r) const {
+    if (warps == 2) return r[0] + r[1];
+    float t = 0.f;
+    for (int i = 0; i < warps; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(r + i);
+      t += (v.x + v.y) + (v.z + v.w);
     }
-    __syncthreads();
-    n = mean = m2 = 0.f;
-    for (int i = 0; i < warps; ++i) merge(n, mean, m2, r[warp0 + i], r[32 + warp0 + i], r[64 + warp0 + i]);
-  }
-  static __device__ __forceinline__ void merge(float& n, float& mean, float& m2, float n2, float mean2, float m22) {
-    const float t = n + n2;
-    const float f = t > 0.f ? n2 / t : 0.f;
-    const float d = mean2 - mean;
-    m2 += m22 + d * d * n * f;
-    mean = fmaf(d, f, mean);
-    n = t;
+    return t;
   }
 };
 
@@ -92,48 +73,102 @@ struct Stat {
   }
 };
 
-// 1 / sqrt(mean square + eps), or with LN the mean and 1 / sqrt(variance + eps), of a row.
+// Rows on their way into shared memory, each thread's vectors at places of its own, so that a thread has
+// nothing but its own copies to wait for.
+template <typename T, int VEC>
+__device__ __forceinline__ void copy_ahead(Raw<T, VEC>* to, const T* from) {
+  constexpr int BYTES = VEC * static_cast<int>(sizeof(T));
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else if constexpr (BYTES == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else
+    *to = ld_raw<T, VEC>(from);
+}
+// Ends a group of copies, and waits until at most `left` groups are under way.
+__device__ __forceinline__ void end_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void wait_copies(int left) {
+  if (left == 2)
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (left == 1)
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// A thread's values of a row, as pairs: NV vectors of VEC, the k-th at column (lane + k tpr) VEC.
+template <int N>
+struct Values {
+  float2 p[N / 2];
+  __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) p[i] = make_float2(v, v);
+  }
+  template <typename T, int VEC>
+  __device__ __forceinline__ void put(int k, const Raw<T, VEC>& r) {
+    float v[VEC];
+    unpack<T, VEC>(r, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) at(k * VEC + e) = v[e];
+  }
+  template <typename T, int VEC>
+  __device__ __forceinline__ Raw<T, VEC> get(int k) const {
+    float v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (k * VEC + e) % 2 ? p[(k * VEC + e) / 2].y : p[(k * VEC + e) / 2].x;
+    return pack<T, VEC>(v);
+  }
+
+ private:
+  __device__ __forceinline__ float& at(int i) { return i % 2 ? p[i / 2].y : p[i / 2].x; }
+};
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// 1 / sqrt(mean square + eps), or with LN the mean and 1 / sqrt(variance + eps), of a row whose values
+// behind its end are 0; inv = 1 / cols.  The variance is taken around the mean in a second reduction: a mean that is large
+// against the deviation cancels nothing.
 template <int VEC, int NV, bool LN>
-__device__ __forceinline__ Stat row_stat(RowGroup& g, const float (&v)[NV][VEC], int cols, float eps) {
-  if constexpr (!LN) {
-    float s = 0.f;
+__device__ __forceinline__ Stat row_stat(RowGroup& g, const float (&v)[NV][VEC], int cols, float inv, float eps) {
+  float s = 0.f, mean = 0.f;
+  if constexpr (LN) {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s = fmaf(v[k][e], v[k][e], s);  // zeros behind the row's end
-    g.sum(s);
-    return {rsqrtf(s / cols + eps), 0.f};
-  } else {
-    float n = 0.f, mean = 0.f, m2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if ((g.lane + k * g.tpr) * VEC < cols) {
-        n += VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) mean += v[k][e];
-      }
-    }
-    if (n > 0.f) mean /= n;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if ((g.lane + k * g.tpr) * VEC < cols) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float d = v[k][e] - mean;
-          m2 = fmaf(d, d, m2);
-        }
-      }
-    }
-    g.join(n, mean, m2);
-    return {rsqrtf(m2 / cols + eps), mean};
+      for (int e = 0; e < VEC; ++e) mean += v[k][e];
+    g.sum(mean);
+    mean *= inv;
   }
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (!LN || (g.lane + k * g.tpr) * VEC < cols) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = v[k][e] - mean;
+        s = fmaf(d, d, s);
+      }
+    }
+  }
+  g.sum(s);
+  return {rsqrtf(fmaf(s, inv, eps)), mean};
 }
 
 constexpr int kMaxCols = 8192;
 constexpr int kMaxThreads = 512;
 
 // Calls go.run<T, VEC, NV, LN>(threads a row) for the widest access that divides the rows' width and
-// their starts (16 bytes, else 4, else one value), with as few vectors a thread as the width allows.
+// their starts (16 bytes, else 4, else one value), with Go::kValues values a thread (VEC at least), or
+// twice as many where kMaxThreads threads are too few for that.
+template <typename T, bool LN, int VEC, typename Go>
+void dispatch_row_width(const Go& go, int cols) {
+  constexpr int NV = Go::kValues > VEC ? Go::kValues / VEC : 1;
+  auto threads = [&](int values) {
+    int t = 32;
+    while (t * values < cols) t *= 2;
+    return t;
+  };
+  if (cols <= kMaxThreads * NV * VEC) return go.template run<T, VEC, NV, LN>(threads(NV * VEC));
+  if constexpr (kMaxThreads * NV * VEC < kMaxCols) go.template run<T, VEC, 2 * NV, LN>(threads(2 * NV * VEC));
+}
 template <typename T, bool LN, typename Go>
 void dispatch_row_vec(const Go& go, const void* const* rows, int n, int cols) {
   constexpr int E = static_cast<int>(sizeof(T));
@@ -143,28 +178,11 @@ void dispatch_row_vec(const Go& go, const void* const* rows, int n, int cols) {
       if (reinterpret_cast<uintptr_t>(rows[i]) % (vec * E)) return false;
     return true;
   };
-  auto threads = [&](int per_thread) {
-    int t = 32;
-    while (t * per_thread < cols) t *= 2;
-    return t;
-  };
-  constexpr int W = 16 / E;
-  constexpr int kNarrow = Go::kOneVector, kMiddle = Go::kTwoVectors;  // in threads a row
-  if (fits(W)) {
-    if (cols <= W * kNarrow) return go.template run<T, W, 1, LN>(threads(W));
-    if constexpr (W * 2 * kMiddle < kMaxCols) {
-      if (cols > W * 2 * kMiddle) return go.template run<T, W, 4, LN>(threads(4 * W));
-    }
-    return go.template run<T, W, 2, LN>(threads(2 * W));
-  }
+  if (fits(16 / E)) return dispatch_row_width<T, LN, 16 / E>(go, cols);
   if constexpr (E == 2) {
-    if (fits(2)) {
-      if (cols <= 2048) return go.template run<T, 2, 4, LN>(threads(8));
-      return go.template run<T, 2, 8, LN>(threads(16));
-    }
+    if (fits(2)) return dispatch_row_width<T, LN, 2>(go, cols);
   }
-  if (cols <= 1024) return go.template run<T, 1, 4, LN>(threads(4));
-  return go.template run<T, 1, 16, LN>(threads(16));
+  dispatch_row_width<T, LN, 1>(go, cols);
 }
 
 template <typename Go>

@@ -5,18 +5,29 @@
 //   dw_pre = sum dn h^, db_pre = sum dn, dw_post = sum dp y^, db_post = sum dp,
 //   dgate = branch_scale sum dH p over the rows that share the gate
 //
-// with h^, y^ the normalised rows (recomputed from h, y and the forward's statistics) and the means
-// in [] for layer norms alone.
+// with the means in [] for layer norms alone.  y^ and h^ are the normalised rows, from y, x and the
+// forward's statistics: h is formed again from x and y rather than read back, the same bytes without
+// the rounding of the stored h.
 //
-// Bound by memory: dh, dn, h and y are read once, dx and dy written once.  A worker (a group of
-// threads that shares a row) walks over a run of rows; its sums over rows stay in shared memory,
-// each thread's columns its own, and leave once, as one partial row a worker (one a run for the
-// gate).  A second kernel adds the partials in a fixed order, so that equal calls give equal bits.
+// Where rows share a gate, its gradient and that of the post norm come from the same column sums A =
+// sum dH y^ and B = sum dH over those rows: dgate = branch_scale (w_post A + b_post B), dw_post +=
+// branch_scale gate A, db_post += branch_scale gate B.
+//
+// Bound by memory: dh, dn, x and y are read once, dx and dy written once.  A worker (a group of
+// threads that shares a row) walks over a run of rows, whose data are copied ahead into shared memory,
+// each thread its own vectors, so that two rows are on their way while one goes through its two
+// reductions.  Sums over rows stay in registers, 8 columns a thread (16 for the widest rows), and leave
+// once, as one partial row a worker (one a run for the gate).  A second kernel adds the partials in a fixed
+// order, so that equal calls give equal bits.  8192 x 4096 bf16 with both norms and a gate: 102 us and 5.5
+// for the sums (403 MB, 61 % of the copy rate).  The arithmetic, through packed fp32 instructions, and the
+// two reductions take about as long as the copies (152 us with unpacked ones, and the sums in shared
+// memory).
 #include <algorithm>
 #include <stdexcept>
 #include <string>
 
 #include "block_norm.cuh"
+#include "tc_common.cuh"
 
 namespace mmf {
 
@@ -24,8 +35,8 @@ namespace {
 
 // Rows are dealt out in chunks of `chunk_rows` that do not cross a gate's group of rows.
 struct Plan {
-  int64_t groups, group_rows;  // rows that share a gate (one group where no sum over rows is asked)
-  int64_t per_group, chunk_rows, chunks;
+  int groups, group_rows;  // of rows that share a gate (one group of all rows where none is shared)
+  int per_group, chunk_rows, chunks;
 };
 
 struct BwdParts {
@@ -33,234 +44,360 @@ struct BwdParts {
   float* gate;                              // [chunks][cols], or null
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_or_zero(const T* p, float* v) {
-  if (p) {
-    unpack<T, VEC>(ld_raw<T, VEC>(p), v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = 0.f;
-  }
-}
-
-// The columns' sums of one thread, in shared memory: array i's vector k of thread `lane`.  Vectors
-// of 8 are split into two of 4 so that a warp's accesses cover whole lines of banks.
-template <int VEC, int NV>
-struct Sums {
-  static constexpr int P = VEC < 4 ? VEC : 4;  // values an access
-  float* base;
-  int tpr, lane;
-  __device__ __forceinline__ float* at(int i, int k, int part) const {
-    return base + (((i * NV + k) * (VEC / P) + part) * tpr + lane) * P;
-  }
-  __device__ __forceinline__ void add(int i, int k, const float* v) const {
-#pragma unroll
-    for (int q = 0; q < VEC / P; ++q) {
-      float* s = at(i, k, q);
-      float t[P];
-      *reinterpret_cast<Raw<float, P>*>(t) = *reinterpret_cast<const Raw<float, P>*>(s);
-#pragma unroll
-      for (int e = 0; e < P; ++e) t[e] += v[q * P + e];
-      *reinterpret_cast<Raw<float, P>*>(s) = *reinterpret_cast<const Raw<float, P>*>(t);
-    }
-  }
-  __device__ __forceinline__ void zero(int i, int cols) const {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int q = 0; q < VEC / P; ++q)
-#pragma unroll
-        for (int e = 0; e < P; ++e) at(i, k, q)[e] = 0.f;
-  }
-  __device__ __forceinline__ void flush(int i, float* dst, int cols) const {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (lane + k * tpr) * VEC;
-      if (c < cols) {
-#pragma unroll
-        for (int q = 0; q < VEC / P; ++q)
-          *reinterpret_cast<Raw<float, P>*>(dst + c + q * P) = *reinterpret_cast<const Raw<float, P>*>(at(i, k, q));
-      }
-    }
-  }
-};
-
-enum { S_POST_W, S_PRE_W, S_GATE, S_POST_B, S_PRE_B };
+// What a stage of the copies holds.
+enum { IN_DN, IN_DH, IN_X, IN_Y, IN_GATE, INPUTS };
 
 template <typename T, int VEC, int NV, bool LN>
-__global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(const BlockNormBwdArgs a, const Plan plan,
-                                                                     const BwdParts parts, int tpr) {
-  extern __shared__ __align__(16) float smem[];
-  __shared__ float red[2 * 3 * 32];
+__global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const BlockNormBwdArgs a, const Plan plan,
+                                                                        const BwdParts parts, int tpr, int stages) {
+  constexpr int N = NV * VEC, H = N / 2;
+  // whether y^ and h^ stay in registers from one reduction to the next and the weights from row to row,
+  // or are formed from the copies and loaded again (for 16 columns a thread there is no room)
+  constexpr bool KEEP = N <= 8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ __align__(16) float red[2 * 2 * 32];
+  using R = Raw<T, VEC>;
+  using V = Values<N>;
   RowGroup g(tpr, red);
-  const int cols = a.cols;
-  const int groups = blockDim.x / tpr;
-  const int64_t worker = static_cast<int64_t>(blockIdx.x) * groups + g.row;
-  const int64_t workers = static_cast<int64_t>(gridDim.x) * groups;
-  const Sums<VEC, NV> sums{smem + static_cast<int64_t>(g.row) * (LN ? 5 : 3) * NV * VEC * tpr, tpr, g.lane};
-#pragma unroll
-  for (int i = 0; i < (LN ? 5 : 3); ++i) sums.zero(i, cols);
-
+  const int cols = a.cols, threads = static_cast<int>(blockDim.x);
+  const int groups = threads / tpr;
+  const int worker = static_cast<int>(blockIdx.x) * groups + g.row, workers = static_cast<int>(gridDim.x) * groups;
   const T* pw = static_cast<const T*>(a.post_w);
   const T* pb = static_cast<const T*>(a.post_b);
   const T* nw = static_cast<const T*>(a.pre_w);
-  const T* gate0 = static_cast<const T*>(a.gate);
-  const float inv = 1.f / cols;
-  const int64_t rounds = (plan.chunks + workers - 1) / workers;
-  for (int64_t round = 0; round < rounds; ++round) {
-    const int64_t chunk = round * workers + worker;
-    const int64_t group = chunk / plan.per_group;
-    const int64_t r0 = (chunk - group * plan.per_group) * plan.chunk_rows;  // within the group
-    for (int64_t i = 0; i < plan.chunk_rows; ++i) {  // the same count for every worker of the block
-      const bool live = chunk < plan.chunks && r0 + i < plan.group_rows;
-      const int64_t row = live ? group * plan.group_rows + r0 + i : 0;
-      const int64_t off = row * cols;
-      const T* gate = gate0 ? gate0 + row / a.rows_per_gate * cols : nullptr;
-      const Stat sh = (live && nw) ? Stat::load<LN>(a.stat_h, row) : Stat{0.f, 0.f};
-      const Stat sy = (live && pw) ? Stat::load<LN>(a.stat_y, row) : Stat{0.f, 0.f};
-      using R = Raw<T, VEC>;
-      R rn[NV], rh[NV], ry[NV];
-      float d[NV][VEC];  // dH
+  const bool gated = a.gate != nullptr, token_gate = gated && a.rows_per_gate == 1;
+  const T* in[INPUTS] = {static_cast<const T*>(nw ? a.dn : nullptr), static_cast<const T*>(a.dh),
+                         static_cast<const T*>(nw ? a.x : nullptr), static_cast<const T*>(pw || gated || nw ? a.y : nullptr),
+                         static_cast<const T*>(token_gate ? a.gate : nullptr)};
+  // stage s's vector k of input i is place(s)[(i * NV + k) * threads]; what is not copied there is 0
+  auto place = [&](int stage) { return reinterpret_cast<R*>(smem) + threadIdx.x + stage * (INPUTS * NV) * threads; };
+  auto clear = [&](int stage) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (g.lane + k * tpr) * VEC;
-        if (live && c < cols) {
-          if (nw) {
-            rn[k] = ld_raw<T, VEC>(static_cast<const T*>(a.dn) + off + c);
-            rh[k] = ld_raw<T, VEC>(static_cast<const T*>(a.h) + off + c);
-          }
-          if (pw || gate) ry[k] = ld_raw<T, VEC>(static_cast<const T*>(a.y) + off + c);
-          load_or_zero<T, VEC>(a.dh ? static_cast<const T*>(a.dh) + off + c : nullptr, d[k]);
-        } else {
+    for (int i = 0; i < INPUTS * NV; ++i) place(stage)[i * threads] = R{};
+  };
+  for (int i = 0; i < stages; ++i) clear(i);
+  auto col = [&](int k) { return (g.lane + k * tpr) * VEC; };
+
+  // the worker's rows: chunk after chunk, as many turns for every worker of the block
+  const int rounds = (plan.chunks + workers - 1) / workers;
+  const int turns = rounds * plan.chunk_rows;
+  struct Cursor {
+    int chunk, i, first, rows;  // row first + i of the chunk's `rows`; none behind the last chunk
+  };
+  auto start = [&](int chunk) {
+    const int group = chunk / plan.per_group;
+    const int at = (chunk - group * plan.per_group) * plan.chunk_rows;  // within the group
+    return Cursor{chunk, 0, group * plan.group_rows + at,
+                  chunk < plan.chunks ? min(plan.chunk_rows, plan.group_rows - at) : 0};
+  };
+  auto step = [&](Cursor& c) {
+    if (++c.i == plan.chunk_rows) c = start(c.chunk + workers);
+  };
+  Cursor ahead = start(worker), now = ahead;
+  int put = 0, get = 0;  // stages
+  auto copy = [&](int turn) {
+    if (turn < turns) {
+      if (ahead.i < ahead.rows) {
+        const int64_t off = static_cast<int64_t>(ahead.first + ahead.i) * cols + g.lane * VEC;
+        R* to = place(put);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[k][e] = 0.f;
-        }
-      }
-      if (nw) {
-        float s1 = 0.f, s2 = 0.f;
+        for (int i = 0; i < INPUTS; ++i) {
+          if (in[i]) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int c = (g.lane + k * tpr) * VEC;
-          if (live && c < cols) {
-            float w[VEC], n[VEC], h[VEC], t[VEC];
-            unpack<T, VEC>(ld_raw<T, VEC>(nw + c), w);
-            unpack<T, VEC>(rn[k], n);
-            unpack<T, VEC>(rh[k], h);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const float u = (h[e] - sh.mean) * sh.rstd;
-              t[e] = n[e] * u;
-              s1 = fmaf(n[e], w[e], s1);
-              s2 = fmaf(t[e], w[e], s2);
-            }
-            if (parts.pre_w) sums.add(S_PRE_W, k, t);
-            if (LN && parts.pre_b) sums.add(S_PRE_B, k, n);
+            for (int k = 0; k < NV; ++k)
+              if (col(k) < cols) copy_ahead<T, VEC>(to + (i * NV + k) * threads, in[i] + off + k * tpr * VEC);
           }
         }
-        g.sum(s2, LN ? &s1 : nullptr);
-        s1 *= inv;
-        s2 *= inv;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int c = (g.lane + k * tpr) * VEC;
-          if (live && c < cols) {
-            float w[VEC], n[VEC], h[VEC];
-            unpack<T, VEC>(ld_raw<T, VEC>(nw + c), w);
-            unpack<T, VEC>(rn[k], n);
-            unpack<T, VEC>(rh[k], h);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const float u = (h[e] - sh.mean) * sh.rstd;
-              d[k][e] += sh.rstd * (n[e] * w[e] - u * s2 - (LN ? s1 : 0.f));
-            }
-          }
-        }
+      } else {
+        clear(put);
       }
-      float s1 = 0.f, s2 = 0.f;
+      step(ahead);
+      if (++put == stages) put = 0;
+    }
+    end_copies();  // one group a turn, empty or not
+  };
+  // a column vector (1 where there is none), 0 behind the row's end
+  auto column = [&](const void* p, V& v) {
+    v.fill(1.f);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (g.lane + k * tpr) * VEC;
-        if (live && c < cols) {
-          float t[VEC], u[VEC], w[VEC], gt[VEC];
-          if (a.dx) {
+    for (int k = 0; k < NV; ++k) {
+      if (col(k) >= cols)
+        v.template put<T, VEC>(k, R{});
+      else if (p)
+        v.template put<T, VEC>(k, ld_raw<T, VEC>(static_cast<const T*>(p) + col(k)));
+    }
+  };
+  auto flush = [&](const V& v, float* to) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) t[e] = a.residual_scale * d[k][e];
-            st_raw<T, VEC>(static_cast<T*>(a.dx) + off + c, pack<T, VEC>(t));
-          }
-          if (pw || gate) unpack<T, VEC>(ry[k], u);
-          if (gate) unpack<T, VEC>(ld_raw<T, VEC>(gate + c), gt);
-          if (pw) unpack<T, VEC>(ld_raw<T, VEC>(pw + c), w);
+    for (int k = 0; k < NV; ++k) {
+      if (col(k) < cols) {
+        constexpr int P = VEC < 4 ? VEC : 4;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            d[k][e] *= a.branch_scale;
-            if (pw) u[e] = (u[e] - sy.mean) * sy.rstd;
-          }
-          if (gate && a.dgate) {
+        for (int e = 0; e < VEC; e += P) {
+          float f[P];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) t[e] = pw ? u[e] * w[e] : u[e];
-            if (LN && pb) {
-              float bb[VEC];
-              unpack<T, VEC>(ld_raw<T, VEC>(pb + c), bb);
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) t[e] += bb[e];
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) t[e] *= d[k][e];
-            if (parts.gate)
-              sums.add(S_GATE, k, t);
-            else
-              st_raw<T, VEC>(static_cast<T*>(a.dgate) + off + c, pack<T, VEC>(t));
-          }
-          if (gate) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) d[k][e] *= gt[e];
-          }
-          if (pw) {
-            if (LN && parts.post_b) sums.add(S_POST_B, k, d[k]);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) t[e] = d[k][e] * u[e];
-            if (parts.post_w) sums.add(S_POST_W, k, t);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              d[k][e] *= w[e];
-              s1 += d[k][e];
-              s2 = fmaf(t[e], w[e], s2);
-            }
-          }
-        }
-      }
-      if (pw) {
-        g.sum(s2, LN ? &s1 : nullptr);
-        s1 *= inv;
-        s2 *= inv;
-      }
-      if (a.dy) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int c = (g.lane + k * tpr) * VEC;
-          if (live && c < cols) {
-            if (pw) {
-              float u[VEC];
-              unpack<T, VEC>(ry[k], u);
-#pragma unroll
-              for (int e = 0; e < VEC; ++e)
-                d[k][e] = sy.rstd * (d[k][e] - (u[e] - sy.mean) * sy.rstd * s2 - (LN ? s1 : 0.f));
-            }
-            st_raw<T, VEC>(static_cast<T*>(a.dy) + off + c, pack<T, VEC>(d[k]));
-          }
+          for (int o = 0; o < P; ++o) f[o] = (k * VEC + e + o) % 2 ? v.p[(k * VEC + e + o) / 2].y : v.p[(k * VEC + e + o) / 2].x;
+          st_raw<float, P>(to + col(k) + e, pack<float, P>(f));
         }
       }
     }
-    if (parts.gate && chunk < plan.chunks) {
-      sums.flush(S_GATE, parts.gate + chunk * cols, cols);
-      sums.zero(S_GATE, cols);
-    }
+  };
+
+  V sum_a, sum_n, sum_pw;
+  [[maybe_unused]] V sum_b, sum_nb, sum_pb;
+  sum_a.fill(0.f);
+  sum_n.fill(0.f);
+  sum_pw.fill(0.f);
+  if constexpr (LN) {
+    sum_b.fill(0.f);
+    sum_nb.fill(0.f);
+    sum_pb.fill(0.f);
   }
-  const int64_t at = worker * cols;
-  if (parts.post_w) sums.flush(S_POST_W, parts.post_w + at, cols);
-  if (parts.pre_w) sums.flush(S_PRE_W, parts.pre_w + at, cols);
-  if (LN && parts.post_b) sums.flush(S_POST_B, parts.post_b + at, cols);
-  if (LN && parts.pre_b) sums.flush(S_PRE_B, parts.pre_b + at, cols);
+  // branch_scale gate times the post norm's weight (d h / d y^), or times its bias (0 where there is none)
+  auto times = [&](const V& gate, const T* p, V& to) {
+    column(p, to);
+#pragma unroll
+    for (int i = 0; i < H; ++i) to.p[i] = fmul2(both(a.branch_scale), fmul2(gate.p[i], to.p[i]));
+  };
+  [[maybe_unused]] V kept_pre, kept_scale, kept_shift;
+  if constexpr (KEEP) column(nw, kept_pre);
+  const float inv = 1.f / cols;
+  const int rows_per_gate = static_cast<int>(a.rows_per_gate);
+  auto load_stats = [&](const Cursor& c, Stat& y, Stat& h) {
+    const bool there = c.i < c.rows;
+    y = there && pw ? Stat::load<LN>(a.stat_y, c.first + c.i) : Stat{1.f, 0.f};
+    h = there && nw ? Stat::load<LN>(a.stat_h, c.first + c.i) : Stat{0.f, 0.f};
+  };
+  Stat next_y, next_h;
+  load_stats(now, next_y, next_h);
+  // with one stage a row's copies start when the row before has been read, else a turn or two earlier
+  for (int i = 0; i < stages - 1; ++i) copy(i);
+  for (int turn = 0; turn < turns; ++turn) {
+    copy(turn + stages - 1);
+    wait_copies(stages - 1);
+    const bool on = now.i < now.rows;
+    const int row = on ? now.first + now.i : 0;
+    const int64_t off = static_cast<int64_t>(row) * cols;
+    const R* here = place(get);
+    auto input = [&](int i, V& v) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) v.template put<T, VEC>(k, here[(i * NV + k) * threads]);
+    };
+    auto store = [&](void* to, const V& v) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (on && col(k) < cols) st_raw<T, VEC>(static_cast<T*>(to) + off + col(k), v.template get<T, VEC>(k));
+    };
+    auto load_gate = [&](V& gate) {
+      if (token_gate)
+        input(IN_GATE, gate);
+      else
+        column(gated ? static_cast<const T*>(a.gate) + static_cast<int64_t>(row / rows_per_gate) * cols : nullptr, gate);
+    };
+    if constexpr (KEEP) {
+      if (token_gate || now.i == 0) {
+        V gate;
+        load_gate(gate);
+        times(gate, pw, kept_scale);
+        if constexpr (LN) times(gate, pb, kept_shift);
+      }
+    }
+    auto load_scale = [&](V& v) {
+      if constexpr (KEEP) {
+        v = kept_scale;
+      } else {
+        V gate;
+        load_gate(gate);
+        times(gate, pw, v);
+      }
+    };
+    auto load_shift = [&](V& v) {
+      if constexpr (KEEP) {
+        v = kept_shift;
+      } else {
+        V gate;
+        load_gate(gate);
+        times(gate, pb, v);
+      }
+    };
+    auto load_pre = [&](V& v) {
+      if constexpr (KEEP)
+        v = kept_pre;
+      else
+        column(nw, v);
+    };
+    // the next row's statistics are on their way while this one's are used
+    const Stat sy = next_y, sh = next_h;
+    Cursor after = now;
+    step(after);
+    load_stats(after, next_y, next_h);
+    auto load_y = [&](V& u) {  // y^ (y without a post norm)
+      input(IN_Y, u);
+      if (pw) {
+        const float2 r = both(sy.rstd), m = both(-sy.mean * sy.rstd);
+#pragma unroll
+        for (int i = 0; i < H; ++i) u.p[i] = LN ? ffma2(u.p[i], r, m) : fmul2(u.p[i], r);
+      }
+    };
+    auto load_h = [&](const V& u, V& h) {  // h^
+      V w;
+      load_scale(w);
+#pragma unroll
+      for (int i = 0; i < H; ++i) h.p[i] = fmul2(u.p[i], w.p[i]);
+      if (LN && pb) {
+        load_shift(w);
+#pragma unroll
+        for (int i = 0; i < H; ++i) h.p[i] = fadd2(h.p[i], w.p[i]);
+      }
+      input(IN_X, w);
+      const float2 r = both(sh.rstd), m = both(-sh.mean * sh.rstd), rho = both(a.residual_scale);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        h.p[i] = ffma2(rho, w.p[i], h.p[i]);
+        h.p[i] = LN ? ffma2(h.p[i], r, m) : fmul2(h.p[i], r);
+      }
+    };
+    V u, d;  // y^; dH, later d h / d (y^)
+    load_y(u);
+    if (nw) {
+      V h, b, pre;
+      load_h(u, h);
+      input(IN_DN, b);
+      load_pre(pre);
+      float2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        sum_n.p[i] = ffma2(b.p[i], h.p[i], sum_n.p[i]);
+        if constexpr (LN) sum_nb.p[i] = fadd2(b.p[i], sum_nb.p[i]);
+        b.p[i] = fmul2(b.p[i], pre.p[i]);
+        if (LN) s1 = fadd2(b.p[i], s1);
+        s2 = ffma2(b.p[i], h.p[i], s2);
+      }
+      float t1 = s1.x + s1.y, t2 = s2.x + s2.y;
+      g.sum(t2, LN ? &t1 : nullptr);
+      input(IN_DH, d);
+      if constexpr (!KEEP) {
+        load_y(u);
+        load_h(u, h);
+        input(IN_DN, b);
+        load_pre(pre);
+#pragma unroll
+        for (int i = 0; i < H; ++i) b.p[i] = fmul2(b.p[i], pre.p[i]);
+      }
+      const float2 r = both(sh.rstd), c2 = both(-sh.rstd * t2 * inv), c1 = both(-sh.rstd * t1 * inv);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        d.p[i] = ffma2(r, b.p[i], d.p[i]);
+        d.p[i] = ffma2(c2, h.p[i], d.p[i]);
+        if (LN) d.p[i] = fadd2(c1, d.p[i]);
+      }
+    } else {
+      input(IN_DH, d);
+    }
+    if (a.dx) {
+      V t;
+#pragma unroll
+      for (int i = 0; i < H; ++i) t.p[i] = fmul2(both(a.residual_scale), d.p[i]);
+      store(a.dx, t);
+    }
+    float2 s1 = both(0.f), s2 = both(0.f);
+    if (token_gate) {
+      // each row's own gate: its gradient goes out with the row, A and B take it in
+      V gate, w, t;
+      input(IN_GATE, gate);
+      column(pw, w);
+      if (a.dgate) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) t.p[i] = fmul2(w.p[i], u.p[i]);
+        if (LN && pb) {
+          V bias;
+          column(pb, bias);
+#pragma unroll
+          for (int i = 0; i < H; ++i) t.p[i] = fadd2(t.p[i], bias.p[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < H; ++i) t.p[i] = fmul2(both(a.branch_scale), fmul2(t.p[i], d.p[i]));
+        store(a.dgate, t);
+      }
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const float2 x = fmul2(d.p[i], gate.p[i]);
+        sum_a.p[i] = ffma2(x, u.p[i], sum_a.p[i]);
+        if constexpr (LN) sum_b.p[i] = fadd2(x, sum_b.p[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        sum_a.p[i] = ffma2(d.p[i], u.p[i], sum_a.p[i]);
+        if constexpr (LN) sum_b.p[i] = fadd2(d.p[i], sum_b.p[i]);
+      }
+    }
+    V scale;
+    load_scale(scale);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      d.p[i] = fmul2(d.p[i], scale.p[i]);
+      if (LN) s1 = fadd2(d.p[i], s1);
+      s2 = ffma2(d.p[i], u.p[i], s2);
+    }
+    if (pw) {
+      float t1 = s1.x + s1.y, t2 = s2.x + s2.y;
+      g.sum(t2, LN ? &t1 : nullptr);
+      if (a.dy) {
+        if constexpr (!KEEP) load_y(u);
+        const float2 r = both(sy.rstd), c2 = both(-sy.rstd * t2 * inv), c1 = both(-sy.rstd * t1 * inv);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          d.p[i] = ffma2(c2, u.p[i], fmul2(r, d.p[i]));
+          if (LN) d.p[i] = fadd2(c1, d.p[i]);
+        }
+      }
+    }
+    if (a.dy) store(a.dy, d);
+
+    if (now.i + 1 == plan.chunk_rows) {  // the chunk's sums
+      V gate, w;
+      if (token_gate) {
+        gate.fill(1.f);
+      } else {
+        const int64_t at = static_cast<int64_t>(now.rows > 0 ? now.first / rows_per_gate : 0) * cols;
+        column(gated ? static_cast<const T*>(a.gate) + at : nullptr, gate);
+      }
+      if (parts.gate && now.chunk < plan.chunks) {
+        V t;
+        column(pw, w);
+#pragma unroll
+        for (int i = 0; i < H; ++i) t.p[i] = fmul2(w.p[i], sum_a.p[i]);
+        if constexpr (LN) {
+          if (pb) {
+            column(pb, w);
+#pragma unroll
+            for (int i = 0; i < H; ++i) t.p[i] = ffma2(w.p[i], sum_b.p[i], t.p[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < H; ++i) t.p[i] = fmul2(both(a.branch_scale), t.p[i]);
+        flush(t, parts.gate + static_cast<int64_t>(now.chunk) * cols);
+      }
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const float2 k = fmul2(both(a.branch_scale), gate.p[i]);
+        sum_pw.p[i] = ffma2(k, sum_a.p[i], sum_pw.p[i]);
+        if constexpr (LN) sum_pb.p[i] = ffma2(k, sum_b.p[i], sum_pb.p[i]);
+      }
+      sum_a.fill(0.f);
+      if constexpr (LN) sum_b.fill(0.f);
+    }
+    now = after;
+    if (++get == stages) get = 0;
+  }
+  const int64_t at = static_cast<int64_t>(worker) * cols;
+  if (parts.post_w) flush(sum_pw, parts.post_w + at);
+  if (parts.pre_w) flush(sum_n, parts.pre_w + at);
+  if constexpr (LN) {
+    if (parts.post_b) flush(sum_pb, parts.post_b + at);
+    if (parts.pre_b) flush(sum_nb, parts.pre_b + at);
+  }
 }
 
 // out[g][c] = sum over i of part[g * n + i][c], in the order of i within each of 8 lanes, then of the
@@ -291,7 +428,7 @@ __global__ void __launch_bounds__(256) block_norm_sum_kernel(const SumJobs jobs,
   float t = 0.f;
   if (c < cols) {
     const float* p = j.part + group * j.n * cols + c;
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t i = threadIdx.y; i < j.n; i += 8) t += p[i * cols];
   }
   s[threadIdx.y][threadIdx.x] = t;
@@ -303,9 +440,11 @@ __global__ void __launch_bounds__(256) block_norm_sum_kernel(const SumJobs jobs,
   }
 }
 
+constexpr int kSharedMost = 224 << 10;
+
 // The launch of a width: what it needs of the device, and how rows are dealt out.
 struct Backward {
-  static constexpr int kOneVector = 128, kTwoVectors = 512;
+  static constexpr int kValues = 8;  // a thread, while the row needs no more than kMaxThreads
   const BlockNormBwdArgs& a;
   cudaStream_t stream;
   int64_t* need;  // non-null: only count the scratch values
@@ -315,30 +454,33 @@ struct Backward {
     auto kernel = block_norm_bwd_kernel<T, VEC, NV, LN>;
     const int block = tpr < 128 ? 128 : tpr;
     const int groups = block / tpr;
-    const int smem = (LN ? 5 : 3) * NV * VEC * tpr * groups * static_cast<int>(sizeof(float));
+    // two rows copied ahead, one or none where they are too wide for that
+    const int stage = INPUTS * NV * VEC * static_cast<int>(sizeof(T)) * block;
+    const int stages = std::max(1, std::min(3, kSharedMost / stage));
+    const int smem = stages * stage;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     int per_sm = 0;
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem);
     if (e != cudaSuccess || per_sm < 1)
       throw std::runtime_error(std::string("mmf: block_norm_bwd: ") + cudaGetErrorString(e));
-    const int64_t most = 148LL * per_sm * groups;  // workers on the device at once
+    const int most = 148 * per_sm * groups;  // workers on the device at once
     Plan p;
-    const bool gate_sum = a.dgate && a.rows_per_gate > 1;
-    p.groups = gate_sum ? a.rows / a.rows_per_gate : 1;
-    p.group_rows = gate_sum ? a.rows_per_gate : a.rows;
+    const bool shared_gate = a.gate && a.rows_per_gate > 1, gate_sum = shared_gate && a.dgate;
+    p.groups = static_cast<int>(shared_gate ? a.rows / a.rows_per_gate : 1);
+    p.group_rows = static_cast<int>(shared_gate ? a.rows_per_gate : a.rows);
     // one chunk a worker while the groups are few; with many groups several smaller ones, so that
     // the last round is not mostly idle
-    p.per_group = p.groups * 4 <= most ? most / p.groups : (4 * most + p.groups - 1) / p.groups;
+    p.per_group = p.groups <= most / 4 ? most / p.groups : (4 * most - 1) / p.groups + 1;
     p.per_group = std::min(p.per_group, p.group_rows);
     p.chunk_rows = (p.group_rows + p.per_group - 1) / p.per_group;
     p.per_group = (p.group_rows + p.chunk_rows - 1) / p.chunk_rows;
     p.chunks = p.groups * p.per_group;
-    const int64_t workers = std::min(most, (p.chunks + groups - 1) / groups * groups);
+    const int workers = std::min(most, (p.chunks + groups - 1) / groups * groups);
 
     int64_t used = 0;
-    auto take = [&](bool want, int64_t rows) {
+    auto take = [&](bool want, int rows) {
       float* at = want && !need ? a.parts + used : nullptr;
-      if (want) used += rows * a.cols;
+      if (want) used += static_cast<int64_t>(rows) * a.cols;
       return at;
     };
     BwdParts parts;
@@ -351,7 +493,7 @@ struct Backward {
       *need = used;
       return;
     }
-    kernel<<<static_cast<unsigned>(workers / groups), block, smem, stream>>>(a, p, parts, tpr);
+    kernel<<<static_cast<unsigned>(workers / groups), block, smem, stream>>>(a, p, parts, tpr, stages);
     check("block_norm_bwd");
 
     SumJobs jobs{};
@@ -364,19 +506,19 @@ struct Backward {
     add(parts.pre_b, a.dpre_b);
     jobs.gate = {parts.gate, a.dgate, p.per_group};
     // grid.y: the arrays, then the gate's groups; past its limit the gate goes on in more launches
-    int64_t gates = gate_sum ? p.groups : 0;
+    int gates = gate_sum ? p.groups : 0;
     if (jobs.count + gates == 0) return;
     const dim3 threads(32, 8);
     while (true) {
-      const int64_t now = std::min<int64_t>(gates, 32768);
+      const int now = std::min(gates, 32768);
       block_norm_sum_kernel<T>
           <<<dim3((a.cols + 31) / 32, static_cast<unsigned>(jobs.count + now)), threads, 0, stream>>>(jobs, a.cols);
       check("block_norm_bwd (sums)");
       gates -= now;
       if (gates == 0) return;
       jobs.count = 0;
-      jobs.gate.part += now * p.per_group * a.cols;
-      jobs.gate.out = static_cast<T*>(jobs.gate.out) + now * a.cols;
+      jobs.gate.part += static_cast<int64_t>(now) * p.per_group * a.cols;
+      jobs.gate.out = static_cast<T*>(jobs.gate.out) + static_cast<int64_t>(now) * a.cols;
     }
   }
   static void check(const char* what) {
@@ -389,7 +531,8 @@ struct Backward {
 
 void go(const Backward& b) {
   const BlockNormBwdArgs& a = b.a;
-  const void* rows[] = {a.dh, a.dn, a.h, a.y, a.post_w, a.post_b, a.gate, a.pre_w, a.dx, a.dy, a.dgate};
+  if (a.rows > 0x3fffffff) throw std::runtime_error("mmf: block_norm_bwd: too many rows");
+  const void* rows[] = {a.dh, a.dn, a.x, a.y, a.post_w, a.post_b, a.gate, a.pre_w, a.dx, a.dy, a.dgate};
   dispatch_row_kernel(b, rows, 11, a.cols, a.dtype, a.layer);
 }
 

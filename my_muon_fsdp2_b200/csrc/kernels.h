@@ -363,7 +363,7 @@ void block_norm_fwd(const BlockNormArgs& args, cudaStream_t stream);
 // Its backward: dx, dy and the gradients of the weights, biases and gate (null: not wanted).
 // dn and dh may each be null (zero).  parts: fp32 scratch of block_norm_bwd_parts(...) values.
 struct BlockNormBwdArgs {
-  const void *dh, *dn, *h, *y, *post_w, *post_b, *gate, *pre_w;
+  const void *dh, *dn, *x, *y, *post_w, *post_b, *gate, *pre_w;
   const float *stat_y, *stat_h;
   void *dx, *dy, *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
   float* parts;
