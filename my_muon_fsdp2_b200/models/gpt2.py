@@ -10,11 +10,12 @@ and the tied head fused with the cross entropy.  ``configure_fsdp`` shards every
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 
+from ..ops.distill import fused_linear_distillation
 from ..ops.linear import gelu_mlp, linear
 from ..ops.model_ops import causal_attention, embedding, fused_linear_cross_entropy, gelu, layer_norm
 
@@ -125,7 +126,11 @@ class GPTModel(nn.Module):
             if getattr(m, "bias", None) is not None:
                 nn.init.zeros_(m.bias)
 
-    def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None):
+    def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
+                teacher: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, temperature: float = 1.0,
+                alpha: float = 1.0):
+        """Logits, or with ``targets`` the mean cross entropy, or with ``teacher`` = (ids, logits), each
+        [batch, seq, top], the mean distillation loss (``ops.distill``)."""
         B, T = input_ids.shape
         if T > self.config.n_positions:
             raise ValueError(f"Sequence length {T} exceeds maximum {self.config.n_positions}")
@@ -134,6 +139,8 @@ class GPTModel(nn.Module):
         for blk in self.h:
             x = blk(x)
         x = self.ln_f(x)
+        if teacher is not None:
+            return fused_linear_distillation(x, self.wte.weight, *teacher, targets, temperature=temperature, alpha=alpha)
         if targets is None:
             return x @ self.wte.weight.t()
         return fused_linear_cross_entropy(x, self.wte.weight, targets)

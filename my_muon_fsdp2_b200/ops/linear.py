@@ -6,7 +6,7 @@ GEMMs of a training step (forward, input gradient, weight gradient), is one laun
 grouped kernel, with the elementwise neighbours fused into its epilogue:
 
 * ``qkv_rope``        q | k | v in one launch (three column segments), RoPE applied to q and k
-                      in the epilogue; backward: one input-gradient launch over the three
+                      in the epilogue (or not at all, where ``ops.rotary`` does it); backward: one input-gradient launch over the three
                       reduction segments, one weight-gradient launch over the three row segments.
 * ``swiglu_ffn``      W2 silu(W1 x) (W3 x) + residual: the two CTAs of each pair stage W1 and W3
                       rows of the same hidden units, so gate and up meet in TMEM and the epilogue
@@ -125,8 +125,11 @@ class _QKVRopeFn(torch.autograd.Function):
     def forward(ctx, x2, src, T, hd, theta, *ws):
         if src.needs_gather():
             q, k, v = src.plain_forward(x2)
-            _rope_(q, T, q.shape[1] // hd, hd, theta, False)
-            _rope_(k, T, k.shape[1] // hd, hd, theta, False)
+            if theta is not None:
+                _rope_(q, T, q.shape[1] // hd, hd, theta, False)
+                _rope_(k, T, k.shape[1] // hd, hd, theta, False)
+        elif theta is None:
+            q, k, v = mm_fwd(x2, src.weights(ws))
         else:
             W = src.weights(ws)
             q, k, v = [torch.empty(x2.shape[0], w.shape[0], dtype=x2.dtype, device=x2.device) for w in W]
@@ -140,9 +143,11 @@ class _QKVRopeFn(torch.autograd.Function):
     def backward(ctx, dq, dk, dv):
         x2, *ws = ctx.saved_tensors
         src, T, hd, theta = ctx.src, ctx.T, ctx.hd, ctx.theta
-        dq, dk, dv = dq.contiguous().clone(), dk.contiguous().clone(), dv.contiguous()
-        _rope_(dq, T, dq.shape[1] // hd, hd, theta, True)
-        _rope_(dk, T, dk.shape[1] // hd, hd, theta, True)
+        dq, dk, dv = dq.contiguous(), dk.contiguous(), dv.contiguous()
+        if theta is not None:
+            dq, dk = dq.clone(), dk.clone()
+            _rope_(dq, T, dq.shape[1] // hd, hd, theta, True)
+            _rope_(dk, T, dk.shape[1] // hd, hd, theta, True)
         W = src.weights(ws)
         dx = mm_dx([dq, dk, dv], W) if ctx.needs_input_grad[0] else None
         gw = src.weight_grads([dq, dk, dv], x2, ctx.needs_input_grad[5:8])
@@ -156,9 +161,10 @@ def _rope_torch(x: torch.Tensor, T: int, hd: int, theta: float) -> torch.Tensor:
     return rt(x.view(M // T, T, N // hd, hd), T, theta).reshape(M, N)
 
 
-def qkv_rope(x: torch.Tensor, mods, seq_len: int, head_dim: int, theta: float):
+def qkv_rope(x: torch.Tensor, mods, seq_len: int, head_dim: int, theta: Optional[float]):
     """(rope(x Wq^T), rope(x Wk^T), x Wv^T) for x [..., D] with T = seq_len consecutive tokens per
-    sequence; 2-D results [tokens, heads * head_dim]."""
+    sequence; 2-D results [tokens, heads * head_dim].  ``theta`` None: the products alone, for
+    rotary positions of another form (``ops.rotary``)."""
     x2 = x.reshape(-1, x.shape[-1])
     src = _Source(mods)
     W = [m.weight for m in mods]
@@ -170,6 +176,8 @@ def qkv_rope(x: torch.Tensor, mods, seq_len: int, head_dim: int, theta: float):
         q, k, v = multi_linear(x2, mods)
     else:
         q, k, v = (F.linear(x2, w) for w in W)
+    if theta is None:
+        return q, k, v
     return _rope_torch(q, seq_len, head_dim, theta), _rope_torch(k, seq_len, head_dim, theta), v
 
 

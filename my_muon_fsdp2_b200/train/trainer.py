@@ -43,7 +43,8 @@ def clip_grad_norm(params, max_norm: float) -> torch.Tensor:
 class Trainer:
     def __init__(self, model: nn.Module, optimizers: Sequence, grad_accum: int = 1, device=None,
                  step_timer=None, max_grad_norm: Optional[float] = None, time_steps: bool = False,
-                 keep_gathered: bool = False, time_phases: bool = False):
+                 keep_gathered: bool = False, time_phases: bool = False, temperature: float = 1.0,
+                 alpha: float = 1.0):
         """``max_grad_norm``: clip the global gradient norm before the optimizer steps, as the
         reference trainers do with 1.0 (examples/train_gpt.py:367-371); None disables it.
         ``time_steps``: bracket every step with CUDA events (read by ``last_step_ms`` and
@@ -55,7 +56,10 @@ class Trainer:
         reshards as usual.
         ``time_phases``: CUDA events between the phases of every step (each micro-batch's
         forward and backward, gradient clipping, the optimizer step); ``phase_ms()`` reads the
-        last step's durations.  Events add no work and no synchronisation inside the step."""
+        last step's durations.  Events add no work and no synchronisation inside the step.
+        ``temperature``, ``alpha``: of the distillation loss, for steps that are given a teacher's top
+        logits (models whose forward takes ``teacher``)."""
+        self.temperature, self.alpha = float(temperature), float(alpha)
         self.model = model
         self.max_grad_norm = max_grad_norm
         self.last_grad_norm: Optional[torch.Tensor] = None
@@ -83,7 +87,7 @@ class Trainer:
             for opt in self.optimizers:
                 ctl.attach_optimizer(opt)
 
-    def _micro(self, tokens: torch.Tensor, i: int):
+    def _micro(self, tokens: torch.Tensor, i: int, teacher=None):
         last = i == self.grad_accum - 1
         if self.grad_sync:
             self.model.set_requires_gradient_sync(last)
@@ -94,7 +98,12 @@ class Trainer:
                 self.model.set_reshard_after_backward(last)
         t = tokens[i]
         with nvtx_range(f"trainer/micro_batch_{i}/forward"):
-            loss = self.model(t[:, :-1], t[:, 1:]) / self.grad_accum
+            if teacher is None:
+                loss = self.model(t[:, :-1], t[:, 1:])
+            else:
+                loss = self.model(t[:, :-1], t[:, 1:], teacher=tuple(x[i] for x in teacher),
+                                  temperature=self.temperature, alpha=self.alpha)
+            loss = loss / self.grad_accum
         self._mark(f"forward_{i}")
         with nvtx_range(f"trainer/micro_batch_{i}/backward"):
             loss.backward()
@@ -128,9 +137,10 @@ class Trainer:
             out[name] = out.get(name, 0.0) + a.elapsed_time(b)
         return out
 
-    def step_on_device(self, tokens: torch.Tensor) -> torch.Tensor:
+    def step_on_device(self, tokens: torch.Tensor, teacher=None) -> torch.Tensor:
         """One optimizer step on a device batch [grad_accum, micro_bs, seq+1]; returns the loss
-        (device tensor, no synchronisation)."""
+        (device tensor, no synchronisation).  ``teacher``: a teacher's top (ids, logits) for the
+        predicted tokens, each [grad_accum, micro_bs, seq, top]: the loss is the distillation."""
         if self.time_steps:
             t0 = torch.cuda.Event(enable_timing=True)
             t0.record()
@@ -140,7 +150,7 @@ class Trainer:
         self._mark("start")
         total = None
         for i in range(self.grad_accum):
-            l = self._micro(tokens, i).detach()
+            l = self._micro(tokens, i, teacher).detach()
             total = l if total is None else total + l
         if self.max_grad_norm is not None:
             ctl = getattr(self.model, "_symm_fsdp", None)
@@ -226,7 +236,10 @@ class Trainer:
             out["comm_gbps"] = comm / (ms / 1e3) / 1e9
         return out
 
-    def train_step(self, batch: torch.Tensor) -> float:
-        """End-to-end step from a host batch [grad_accum, micro_bs, seq+1] (int64)."""
+    def train_step(self, batch: torch.Tensor, teacher=None) -> float:
+        """End-to-end step from a host batch [grad_accum, micro_bs, seq+1] (int64), and with
+        distillation the teacher's top (ids, logits) as in ``step_on_device``."""
         tokens = batch.to(self.device, non_blocking=True)
-        return float(self.step_on_device(tokens).item())
+        if teacher is not None:
+            teacher = tuple(x.to(self.device, non_blocking=True) for x in teacher)
+        return float(self.step_on_device(tokens, teacher).item())
