@@ -15,6 +15,7 @@
 #include <string>
 
 #include "block_norm.cuh"
+#include "launch_info.h"
 
 namespace mmf {
 
@@ -161,12 +162,8 @@ struct Forward {
     const int stage = inputs * NV * VEC * static_cast<int>(sizeof(T)) * block;
     const int stages = 3 * stage <= (56 << 10) ? 3 : 2 * stage <= (112 << 10) ? 2 : 1;
     const int smem = stages * stage;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     const int64_t want = (a.rows + groups - 1) / groups;
-    int per_sm = 1;
-    if (e == cudaSuccess && want > 148) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem);
-    if (e != cudaSuccess || per_sm < 1)
-      throw std::runtime_error(std::string("mmf: block_norm: ") + cudaGetErrorString(e));
+    const int per_sm = resident_blocks(reinterpret_cast<const void*>(kernel), block, smem);
     const unsigned blocks = static_cast<unsigned>(want < 148LL * per_sm ? want : 148LL * per_sm);
     kernel<<<blocks, block, smem, stream>>>(a, tpr, inputs, stages);
   }

@@ -27,6 +27,7 @@
 #include <string>
 
 #include "block_norm.cuh"
+#include "launch_info.h"
 #include "tc_common.cuh"
 
 namespace mmf {
@@ -458,11 +459,7 @@ struct Backward {
     const int stage = INPUTS * NV * VEC * static_cast<int>(sizeof(T)) * block;
     const int stages = std::max(1, std::min(3, kSharedMost / stage));
     const int smem = stages * stage;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    int per_sm = 0;
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem);
-    if (e != cudaSuccess || per_sm < 1)
-      throw std::runtime_error(std::string("mmf: block_norm_bwd: ") + cudaGetErrorString(e));
+    const int per_sm = resident_blocks(reinterpret_cast<const void*>(kernel), block, smem);
     const int most = 148 * per_sm * groups;  // workers on the device at once
     Plan p;
     const bool shared_gate = a.gate && a.rows_per_gate > 1, gate_sum = shared_gate && a.dgate;

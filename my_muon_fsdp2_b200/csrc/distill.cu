@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "kernels.h"
+#include "launch_info.h"
 #include "tc_common.cuh"
 #include "typed_io.cuh"
 
@@ -701,10 +702,7 @@ void distill_rows(const DistillArgs& a, cudaStream_t stream) {
     const int each = (a.vocab / Vec<T>::N + blocks - 1) / blocks;
     const int smem = each * 16 + slot_bytes(a.top);
     auto kernel = distill_rows_kernel<T, decltype(mode)::value>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) throw std::runtime_error(std::string("mmf: distill: ") + cudaGetErrorString(e));
+    allow_shared(reinterpret_cast<const void*>(kernel), smem, /*carveout=*/true);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(blocks));
     cfg.blockDim = dim3(kThreads);

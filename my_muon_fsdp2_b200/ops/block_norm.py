@@ -51,14 +51,15 @@ def _check(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, norm) -> No
         raise TypeError(f"gated_residual_norm: x must be bf16, fp16 or fp32, got {x.dtype}")
     if y.shape != x.shape:
         raise ValueError(f"gated_residual_norm: y {tuple(y.shape)} must have x's shape {tuple(x.shape)}")
+    dtype, device, dim = x.dtype, x.device, x.shape[-1:]
     for name, t in (("y", y), ("post_weight", post_weight), ("post_bias", post_bias), ("gate", gate),
                     ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
         if t is None:
             continue
-        if t.dtype != x.dtype or t.device != x.device:
-            raise TypeError(f"gated_residual_norm: {name} must have x's dtype {x.dtype} and device {x.device}")
-        if name not in ("y", "gate") and t.shape != x.shape[-1:]:
-            raise ValueError(f"gated_residual_norm: {name} must be [{x.shape[-1]}], got {tuple(t.shape)}")
+        if t.dtype != dtype or t.device != device:
+            raise TypeError(f"gated_residual_norm: {name} must have x's dtype {dtype} and device {device}")
+        if name not in ("y", "gate") and t.shape != dim:
+            raise ValueError(f"gated_residual_norm: {name} must be [{dim[0]}], got {tuple(t.shape)}")
     for name, b, w in (("post_bias", post_bias, post_weight), ("pre_bias", pre_bias, pre_weight)):
         if b is not None and (w is None or norm != "layer"):
             raise ValueError(f"gated_residual_norm: {name} needs its weight and norm='layer'")
