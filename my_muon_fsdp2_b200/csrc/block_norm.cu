@@ -27,7 +27,7 @@ template <typename T, int VEC, int NV, bool LN>
 __global__ void __launch_bounds__(kMaxThreads) block_norm_fwd_kernel(const BlockNormArgs a, int tpr, int inputs,
                                                                      int stages) {
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ __align__(16) float red[2 * 2 * 32];
+  __shared__ __align__(16) float red[2 * 4 * 32];
   using R = Raw<T, VEC>;
   RowGroup g(tpr, red);
   const int cols = a.cols, threads = static_cast<int>(blockDim.x), groups = threads / tpr;

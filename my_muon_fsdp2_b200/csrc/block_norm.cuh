@@ -16,7 +16,7 @@ namespace {
 // block takes part in every reduction.
 struct RowGroup {
   int tpr, row, lane, warp0, warps;
-  float* red;  // [2][2][32], used in turn so that one barrier a reduction is enough; 16-byte aligned
+  float* red;  // [2][4][32], used in turn so that one barrier a reduction is enough; 16-byte aligned
   int turn = 0;
   __device__ RowGroup(int tpr_, float* red_) : tpr(tpr_), red(red_) {
     row = threadIdx.x / tpr;
@@ -24,24 +24,29 @@ struct RowGroup {
     warps = tpr >> 5;
     warp0 = row * warps;
   }
-  // The sum of a (and of b) over the row's threads, the same bits in each of them.
-  __device__ __forceinline__ void sum(float& a, float* b = nullptr) {
+  // Each of v summed over the row's threads, the same bits in each of them.
+  template <int M>
+  __device__ __forceinline__ void sum(float (&v)[M]) {
+    static_assert(M <= 4, "");
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      if (b) *b += __shfl_xor_sync(0xffffffffu, *b, o);
-    }
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < M; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     if (warps == 1) return;
-    float* r = red + 64 * turn;
+    float* r = red + 128 * turn;
     turn ^= 1;
-    const int w = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) {
-      r[w] = a;
-      if (b) r[32 + w] = *b;
+#pragma unroll
+      for (int i = 0; i < M; ++i) r[32 * i + (threadIdx.x >> 5)] = v[i];
     }
     __syncthreads();
-    a = over_warps(r + warp0);
-    if (b) *b = over_warps(r + 32 + warp0);
+#pragma unroll
+    for (int i = 0; i < M; ++i) v[i] = over_warps(r + 32 * i + warp0);
+  }
+  __device__ __forceinline__ float sum(float v) {
+    float w[1] = {v};
+    sum(w);
+    return w[0];
   }
 
  private:
@@ -135,8 +140,7 @@ __device__ __forceinline__ Stat row_stat(RowGroup& g, const float (&v)[NV][VEC],
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) mean += v[k][e];
-    g.sum(mean);
-    mean *= inv;
+    mean = g.sum(mean) * inv;
   }
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -148,7 +152,7 @@ __device__ __forceinline__ Stat row_stat(RowGroup& g, const float (&v)[NV][VEC],
       }
     }
   }
-  g.sum(s);
+  s = g.sum(s);
   return {rsqrtf(fmaf(s, inv, eps)), mean};
 }
 

@@ -15,13 +15,13 @@
 //
 // Bound by memory: dh, dn, x and y are read once, dx and dy written once.  A worker (a group of
 // threads that shares a row) walks over a run of rows, whose data are copied ahead into shared memory,
-// each thread its own vectors, so that two rows are on their way while one goes through its two
+// each thread its own vectors, so that others are on their way while it is at one or two rows' two
 // reductions.  Sums over rows stay in registers, 8 columns a thread (16 for the widest rows), and leave
 // once, as one partial row a worker (one a run for the gate).  A second kernel adds the partials in a fixed
-// order, so that equal calls give equal bits.  8192 x 4096 bf16 with both norms and a gate: 102 us and 5.5
-// for the sums (403 MB, 61 % of the copy rate).  The arithmetic, through packed fp32 instructions, and the
-// two reductions take about as long as the copies (152 us with unpacked ones, and the sums in shared
-// memory).
+// order, so that equal calls give equal bits.  8192 x 4096 bf16 with both norms and a gate: 97 us, and 5.5
+// for the sums (403 MB, 64 % of the copy rate); the arithmetic, through packed fp32 instructions, takes
+// about as long as the copies.  One row a turn 102 us; unpacked arithmetic, sums in shared memory and
+// no copies ahead 152; 16 columns a thread and two blocks an SM, weights loaded again for each row, 140.
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -48,15 +48,21 @@ struct BwdParts {
 // What a stage of the copies holds.
 enum { IN_DN, IN_DH, IN_X, IN_Y, IN_GATE, INPUTS };
 
+// Rows that a worker takes in one turn (with a layer norm's sums there is no room for two).
+template <int N, bool LN>
+constexpr int kRows = N <= 8 && !LN ? 2 : 1;
+
 template <typename T, int VEC, int NV, bool LN>
 __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const BlockNormBwdArgs a, const Plan plan,
-                                                                        const BwdParts parts, int tpr, int stages) {
+                                                                        const BwdParts parts, int tpr, int inputs,
+                                                                        int stages) {
   constexpr int N = NV * VEC, H = N / 2;
   // whether y^ and h^ stay in registers from one reduction to the next and the weights from row to row,
   // or are formed from the copies and loaded again (for 16 columns a thread there is no room)
   constexpr bool KEEP = N <= 8;
+  constexpr int ROWS = kRows<N, LN>;  // in one turn, so that they share its barriers
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ __align__(16) float red[2 * 2 * 32];
+  __shared__ __align__(16) float red[2 * 4 * 32];
   using R = Raw<T, VEC>;
   using V = Values<N>;
   RowGroup g(tpr, red);
@@ -70,18 +76,21 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   const T* in[INPUTS] = {static_cast<const T*>(nw ? a.dn : nullptr), static_cast<const T*>(a.dh),
                          static_cast<const T*>(nw ? a.x : nullptr), static_cast<const T*>(pw || gated || nw ? a.y : nullptr),
                          static_cast<const T*>(token_gate ? a.gate : nullptr)};
-  // stage s's vector k of input i is place(s)[(i * NV + k) * threads]; what is not copied there is 0
-  auto place = [&](int stage) { return reinterpret_cast<R*>(smem) + threadIdx.x + stage * (INPUTS * NV) * threads; };
-  auto clear = [&](int stage) {
-#pragma unroll
-    for (int i = 0; i < INPUTS * NV; ++i) place(stage)[i * threads] = R{};
+  // stage s's vector k of row r's input i is place(s, r)[(i * NV + k) * threads]; what is not copied there
+  // is 0
+  auto place = [&](int stage, int r) {
+    return reinterpret_cast<R*>(smem) + threadIdx.x + (stage * ROWS + r) * (inputs * NV) * threads;
   };
-  for (int i = 0; i < stages; ++i) clear(i);
+  auto clear = [&](int stage, int r) {
+    for (int i = 0; i < inputs * NV; ++i) place(stage, r)[i * threads] = R{};
+  };
+  for (int i = 0; i < stages; ++i)
+    for (int r = 0; r < ROWS; ++r) clear(i, r);
   auto col = [&](int k) { return (g.lane + k * tpr) * VEC; };
 
   // the worker's rows: chunk after chunk, as many turns for every worker of the block
   const int rounds = (plan.chunks + workers - 1) / workers;
-  const int turns = rounds * plan.chunk_rows;
+  const int turns = rounds * ((plan.chunk_rows + ROWS - 1) / ROWS);
   struct Cursor {
     int chunk, i, first, rows;  // row first + i of the chunk's `rows`; none behind the last chunk
   };
@@ -92,25 +101,28 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
                   chunk < plan.chunks ? min(plan.chunk_rows, plan.group_rows - at) : 0};
   };
   auto step = [&](Cursor& c) {
-    if (++c.i == plan.chunk_rows) c = start(c.chunk + workers);
+    if ((c.i += ROWS) >= plan.chunk_rows) c = start(c.chunk + workers);
   };
   Cursor ahead = start(worker), now = ahead;
   int put = 0, get = 0;  // stages
   auto copy = [&](int turn) {
     if (turn < turns) {
-      if (ahead.i < ahead.rows) {
-        const int64_t off = static_cast<int64_t>(ahead.first + ahead.i) * cols + g.lane * VEC;
-        R* to = place(put);
 #pragma unroll
-        for (int i = 0; i < INPUTS; ++i) {
-          if (in[i]) {
+      for (int r = 0; r < ROWS; ++r) {
+        if (ahead.i + r < ahead.rows) {
+          const int64_t off = static_cast<int64_t>(ahead.first + ahead.i + r) * cols + g.lane * VEC;
+          R* to = place(put, r);
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
-              if (col(k) < cols) copy_ahead<T, VEC>(to + (i * NV + k) * threads, in[i] + off + k * tpr * VEC);
+          for (int i = 0; i < INPUTS; ++i) {
+            if (in[i]) {
+#pragma unroll
+              for (int k = 0; k < NV; ++k)
+                if (col(k) < cols) copy_ahead<T, VEC>(to + (i * NV + k) * threads, in[i] + off + k * tpr * VEC);
+            }
           }
+        } else {
+          clear(put, r);
         }
-      } else {
-        clear(put);
       }
       step(ahead);
       if (++put == stages) put = 0;
@@ -164,60 +176,63 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   if constexpr (KEEP) column(nw, kept_pre);
   const float inv = 1.f / cols;
   const int rows_per_gate = static_cast<int>(a.rows_per_gate);
-  auto load_stats = [&](const Cursor& c, Stat& y, Stat& h) {
-    const bool there = c.i < c.rows;
-    y = there && pw ? Stat::load<LN>(a.stat_y, c.first + c.i) : Stat{1.f, 0.f};
-    h = there && nw ? Stat::load<LN>(a.stat_h, c.first + c.i) : Stat{0.f, 0.f};
+  auto load_stats = [&](const Cursor& c, Stat (&y)[ROWS], Stat (&h)[ROWS]) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const bool there = c.i + r < c.rows;
+      y[r] = there && pw ? Stat::load<LN>(a.stat_y, c.first + c.i + r) : Stat{1.f, 0.f};
+      h[r] = there && nw ? Stat::load<LN>(a.stat_h, c.first + c.i + r) : Stat{0.f, 0.f};
+    }
   };
-  Stat next_y, next_h;
+  Stat next_y[ROWS], next_h[ROWS];
   load_stats(now, next_y, next_h);
-  // with one stage a row's copies start when the row before has been read, else a turn or two earlier
+  // with one stage rows' copies start when those before have been read, else a turn or two earlier
   for (int i = 0; i < stages - 1; ++i) copy(i);
   for (int turn = 0; turn < turns; ++turn) {
     copy(turn + stages - 1);
     wait_copies(stages - 1);
-    const bool on = now.i < now.rows;
-    const int row = on ? now.first + now.i : 0;
-    const int64_t off = static_cast<int64_t>(row) * cols;
-    const R* here = place(get);
-    auto input = [&](int i, V& v) {
+    auto input = [&](int r, int i, V& v) {
+      const R* here = place(get, r);
 #pragma unroll
       for (int k = 0; k < NV; ++k) v.template put<T, VEC>(k, here[(i * NV + k) * threads]);
     };
-    auto store = [&](void* to, const V& v) {
+    auto store = [&](int r, void* to, const V& v) {
+      const int64_t off = static_cast<int64_t>(now.first + now.i + r) * cols;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (on && col(k) < cols) st_raw<T, VEC>(static_cast<T*>(to) + off + col(k), v.template get<T, VEC>(k));
+        if (now.i + r < now.rows && col(k) < cols)
+          st_raw<T, VEC>(static_cast<T*>(to) + off + col(k), v.template get<T, VEC>(k));
     };
-    auto load_gate = [&](V& gate) {
+    auto load_gate = [&](int r, V& gate) {
       if (token_gate)
-        input(IN_GATE, gate);
-      else
-        column(gated ? static_cast<const T*>(a.gate) + static_cast<int64_t>(row / rows_per_gate) * cols : nullptr, gate);
+        input(r, IN_GATE, gate);
+      else  // the chunk's
+        column(gated ? static_cast<const T*>(a.gate) + static_cast<int64_t>(now.rows > 0 ? now.first / rows_per_gate : 0) * cols
+                     : nullptr, gate);
     };
     if constexpr (KEEP) {
-      if (token_gate || now.i == 0) {
+      if (now.i == 0 && !token_gate) {
         V gate;
-        load_gate(gate);
+        load_gate(0, gate);
         times(gate, pw, kept_scale);
         if constexpr (LN) times(gate, pb, kept_shift);
       }
     }
-    auto load_scale = [&](V& v) {
-      if constexpr (KEEP) {
+    auto load_scale = [&](int r, V& v) {
+      if (KEEP && !token_gate) {
         v = kept_scale;
       } else {
         V gate;
-        load_gate(gate);
+        load_gate(r, gate);
         times(gate, pw, v);
       }
     };
-    auto load_shift = [&](V& v) {
-      if constexpr (KEEP) {
+    auto load_shift = [&](int r, V& v) {
+      if (KEEP && !token_gate) {
         v = kept_shift;
       } else {
         V gate;
-        load_gate(gate);
+        load_gate(r, gate);
         times(gate, pb, v);
       }
     };
@@ -227,136 +242,168 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
       else
         column(nw, v);
     };
-    // the next row's statistics are on their way while this one's are used
-    const Stat sy = next_y, sh = next_h;
+    // the next rows' statistics are on their way while these are used
+    Stat sy[ROWS], sh[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      sy[r] = next_y[r];
+      sh[r] = next_h[r];
+    }
     Cursor after = now;
     step(after);
     load_stats(after, next_y, next_h);
-    auto load_y = [&](V& u) {  // y^ (y without a post norm)
-      input(IN_Y, u);
+    auto load_y = [&](int r, V& u) {  // y^ (y without a post norm)
+      input(r, IN_Y, u);
       if (pw) {
-        const float2 r = both(sy.rstd), m = both(-sy.mean * sy.rstd);
+        const float2 s = both(sy[r].rstd), m = both(-sy[r].mean * sy[r].rstd);
 #pragma unroll
-        for (int i = 0; i < H; ++i) u.p[i] = LN ? ffma2(u.p[i], r, m) : fmul2(u.p[i], r);
+        for (int i = 0; i < H; ++i) u.p[i] = LN ? ffma2(u.p[i], s, m) : fmul2(u.p[i], s);
       }
     };
-    auto load_h = [&](const V& u, V& h) {  // h^
+    auto load_h = [&](int r, const V& u, V& h) {  // h^
       V w;
-      load_scale(w);
+      load_scale(r, w);
 #pragma unroll
       for (int i = 0; i < H; ++i) h.p[i] = fmul2(u.p[i], w.p[i]);
       if (LN && pb) {
-        load_shift(w);
+        load_shift(r, w);
 #pragma unroll
         for (int i = 0; i < H; ++i) h.p[i] = fadd2(h.p[i], w.p[i]);
       }
-      input(IN_X, w);
-      const float2 r = both(sh.rstd), m = both(-sh.mean * sh.rstd), rho = both(a.residual_scale);
+      input(r, IN_X, w);
+      const float2 s = both(sh[r].rstd), m = both(-sh[r].mean * sh[r].rstd), rho = both(a.residual_scale);
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         h.p[i] = ffma2(rho, w.p[i], h.p[i]);
-        h.p[i] = LN ? ffma2(h.p[i], r, m) : fmul2(h.p[i], r);
+        h.p[i] = LN ? ffma2(h.p[i], s, m) : fmul2(h.p[i], s);
       }
     };
-    V u, d;  // y^; dH, later d h / d (y^)
-    load_y(u);
-    if (nw) {
-      V h, b, pre;
-      load_h(u, h);
-      input(IN_DN, b);
+    auto load_b = [&](int r, V& b) {  // dn w_pre
+      V pre;
+      input(r, IN_DN, b);
       load_pre(pre);
+#pragma unroll
+      for (int i = 0; i < H; ++i) b.p[i] = fmul2(b.p[i], pre.p[i]);
+    };
+    constexpr int SUMS = LN ? 2 : 1;
+    float t[ROWS * SUMS];
+    V u[ROWS], d[ROWS];  // y^; dn w_pre, then dH, then d h / d (y^)
+    if (nw) {
+      V h[ROWS];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        load_y(r, u[r]);
+        load_h(r, u[r], h[r]);
+        input(r, IN_DN, d[r]);
+        V pre;
+        load_pre(pre);
+        float2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          sum_n.p[i] = ffma2(d[r].p[i], h[r].p[i], sum_n.p[i]);
+          if constexpr (LN) sum_nb.p[i] = fadd2(d[r].p[i], sum_nb.p[i]);
+          d[r].p[i] = fmul2(d[r].p[i], pre.p[i]);
+          if (LN) s1 = fadd2(d[r].p[i], s1);
+          s2 = ffma2(d[r].p[i], h[r].p[i], s2);
+        }
+        t[r * SUMS] = s2.x + s2.y;
+        if constexpr (LN) t[r * SUMS + 1] = s1.x + s1.y;
+      }
+      g.sum(t);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if constexpr (!KEEP) {
+          load_y(r, u[r]);
+          load_h(r, u[r], h[r]);
+          load_b(r, d[r]);
+        }
+        V dh;
+        input(r, IN_DH, dh);
+        const float k = -sh[r].rstd * inv;
+        const float2 s = both(sh[r].rstd), c2 = both(k * t[r * SUMS]);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          d[r].p[i] = ffma2(s, d[r].p[i], dh.p[i]);
+          d[r].p[i] = ffma2(c2, h[r].p[i], d[r].p[i]);
+          if constexpr (LN) d[r].p[i] = fadd2(both(k * t[r * SUMS + 1]), d[r].p[i]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        load_y(r, u[r]);
+        input(r, IN_DH, d[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (a.dx) {
+        V x;
+#pragma unroll
+        for (int i = 0; i < H; ++i) x.p[i] = fmul2(both(a.residual_scale), d[r].p[i]);
+        store(r, a.dx, x);
+      }
+      if (token_gate) {
+        // each row's own gate: its gradient goes out with the row, A and B take it in
+        V gate, w, x;
+        input(r, IN_GATE, gate);
+        if (a.dgate) {
+          column(pw, w);
+#pragma unroll
+          for (int i = 0; i < H; ++i) x.p[i] = fmul2(w.p[i], u[r].p[i]);
+          if (LN && pb) {
+            column(pb, w);
+#pragma unroll
+            for (int i = 0; i < H; ++i) x.p[i] = fadd2(x.p[i], w.p[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < H; ++i) x.p[i] = fmul2(both(a.branch_scale), fmul2(x.p[i], d[r].p[i]));
+          store(r, a.dgate, x);
+        }
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          const float2 x = fmul2(d[r].p[i], gate.p[i]);
+          sum_a.p[i] = ffma2(x, u[r].p[i], sum_a.p[i]);
+          if constexpr (LN) sum_b.p[i] = fadd2(x, sum_b.p[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          sum_a.p[i] = ffma2(d[r].p[i], u[r].p[i], sum_a.p[i]);
+          if constexpr (LN) sum_b.p[i] = fadd2(d[r].p[i], sum_b.p[i]);
+        }
+      }
+      V scale;
+      load_scale(r, scale);
       float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        sum_n.p[i] = ffma2(b.p[i], h.p[i], sum_n.p[i]);
-        if constexpr (LN) sum_nb.p[i] = fadd2(b.p[i], sum_nb.p[i]);
-        b.p[i] = fmul2(b.p[i], pre.p[i]);
-        if (LN) s1 = fadd2(b.p[i], s1);
-        s2 = ffma2(b.p[i], h.p[i], s2);
+        d[r].p[i] = fmul2(d[r].p[i], scale.p[i]);
+        if (LN) s1 = fadd2(d[r].p[i], s1);
+        s2 = ffma2(d[r].p[i], u[r].p[i], s2);
       }
-      float t1 = s1.x + s1.y, t2 = s2.x + s2.y;
-      g.sum(t2, LN ? &t1 : nullptr);
-      input(IN_DH, d);
-      if constexpr (!KEEP) {
-        load_y(u);
-        load_h(u, h);
-        input(IN_DN, b);
-        load_pre(pre);
-#pragma unroll
-        for (int i = 0; i < H; ++i) b.p[i] = fmul2(b.p[i], pre.p[i]);
-      }
-      const float2 r = both(sh.rstd), c2 = both(-sh.rstd * t2 * inv), c1 = both(-sh.rstd * t1 * inv);
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        d.p[i] = ffma2(r, b.p[i], d.p[i]);
-        d.p[i] = ffma2(c2, h.p[i], d.p[i]);
-        if (LN) d.p[i] = fadd2(c1, d.p[i]);
-      }
-    } else {
-      input(IN_DH, d);
+      t[r * SUMS] = s2.x + s2.y;
+      if constexpr (LN) t[r * SUMS + 1] = s1.x + s1.y;
     }
-    if (a.dx) {
-      V t;
+    if (pw) g.sum(t);
+    if (a.dy) {
 #pragma unroll
-      for (int i = 0; i < H; ++i) t.p[i] = fmul2(both(a.residual_scale), d.p[i]);
-      store(a.dx, t);
-    }
-    float2 s1 = both(0.f), s2 = both(0.f);
-    if (token_gate) {
-      // each row's own gate: its gradient goes out with the row, A and B take it in
-      V gate, w, t;
-      input(IN_GATE, gate);
-      column(pw, w);
-      if (a.dgate) {
+      for (int r = 0; r < ROWS; ++r) {
+        if (pw) {
+          if constexpr (!KEEP) load_y(r, u[r]);
+          const float k = -sy[r].rstd * inv;
+          const float2 s = both(sy[r].rstd), c2 = both(k * t[r * SUMS]);
 #pragma unroll
-        for (int i = 0; i < H; ++i) t.p[i] = fmul2(w.p[i], u.p[i]);
-        if (LN && pb) {
-          V bias;
-          column(pb, bias);
-#pragma unroll
-          for (int i = 0; i < H; ++i) t.p[i] = fadd2(t.p[i], bias.p[i]);
+          for (int i = 0; i < H; ++i) {
+            d[r].p[i] = ffma2(c2, u[r].p[i], fmul2(s, d[r].p[i]));
+            if constexpr (LN) d[r].p[i] = fadd2(both(k * t[r * SUMS + 1]), d[r].p[i]);
+          }
         }
-#pragma unroll
-        for (int i = 0; i < H; ++i) t.p[i] = fmul2(both(a.branch_scale), fmul2(t.p[i], d.p[i]));
-        store(a.dgate, t);
-      }
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        const float2 x = fmul2(d.p[i], gate.p[i]);
-        sum_a.p[i] = ffma2(x, u.p[i], sum_a.p[i]);
-        if constexpr (LN) sum_b.p[i] = fadd2(x, sum_b.p[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        sum_a.p[i] = ffma2(d.p[i], u.p[i], sum_a.p[i]);
-        if constexpr (LN) sum_b.p[i] = fadd2(d.p[i], sum_b.p[i]);
+        store(r, a.dy, d[r]);
       }
     }
-    V scale;
-    load_scale(scale);
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      d.p[i] = fmul2(d.p[i], scale.p[i]);
-      if (LN) s1 = fadd2(d.p[i], s1);
-      s2 = ffma2(d.p[i], u.p[i], s2);
-    }
-    if (pw) {
-      float t1 = s1.x + s1.y, t2 = s2.x + s2.y;
-      g.sum(t2, LN ? &t1 : nullptr);
-      if (a.dy) {
-        if constexpr (!KEEP) load_y(u);
-        const float2 r = both(sy.rstd), c2 = both(-sy.rstd * t2 * inv), c1 = both(-sy.rstd * t1 * inv);
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-          d.p[i] = ffma2(c2, u.p[i], fmul2(r, d.p[i]));
-          if (LN) d.p[i] = fadd2(c1, d.p[i]);
-        }
-      }
-    }
-    if (a.dy) store(a.dy, d);
 
-    if (now.i + 1 == plan.chunk_rows) {  // the chunk's sums
+    if (now.i + ROWS >= plan.chunk_rows) {  // the chunk's sums
       V gate, w;
       if (token_gate) {
         gate.fill(1.f);
@@ -456,7 +503,8 @@ struct Backward {
     const int block = tpr < 128 ? 128 : tpr;
     const int groups = block / tpr;
     // two rows copied ahead, one or none where they are too wide for that
-    const int stage = INPUTS * NV * VEC * static_cast<int>(sizeof(T)) * block;
+    const int inputs = a.gate && a.rows_per_gate == 1 ? INPUTS : INPUTS - 1;
+    const int stage = kRows<NV * VEC, LN> * inputs * NV * VEC * static_cast<int>(sizeof(T)) * block;
     const int stages = std::max(1, std::min(3, kSharedMost / stage));
     const int smem = stages * stage;
     const int per_sm = resident_blocks(reinterpret_cast<const void*>(kernel), block, smem);
@@ -490,7 +538,7 @@ struct Backward {
       *need = used;
       return;
     }
-    kernel<<<static_cast<unsigned>(workers / groups), block, smem, stream>>>(a, p, parts, tpr, stages);
+    kernel<<<static_cast<unsigned>(workers / groups), block, smem, stream>>>(a, p, parts, tpr, inputs, stages);
     check("block_norm_bwd");
 
     SumJobs jobs{};
