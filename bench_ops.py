@@ -89,6 +89,30 @@ def cases(E):
     dy_e = torch.randn(T, D, device=dev, dtype=bf)
     out["embedding_bwd"] = (lambda: E.embedding_bwd(dy_e, tok, V), V * D * 2 + T * D * 2, T * D * 2)
 
+    # the same block's rotary positions with scaled frequencies, q and k in one launch; the norms on both
+    # sides of the attention with gate and residual scale; distillation from 64 top logits at tau 2 with
+    # hard targets (loss and gradient in one reading of the logits, in place)
+    from my_muon_fsdp2_b200.ops.block_norm import gated_residual_norm
+    from my_muon_fsdp2_b200.ops.rotary import RopeScaling, RotaryEmbedding, apply_rotary
+
+    rot = RotaryEmbedding(HD, 500000.0, scaling=RopeScaling("llama3", 8.0)).to(dev)
+    q4, k4 = (torch.randn(1, T, h, HD, device=dev, dtype=bf) for h in (H, KV))
+    out["rotary_qk"] = (lambda: apply_rotary(q4, k4, rot), 2 * (q4.numel() + k4.numel()) * 2,
+                        (q4.numel() + k4.numel()) * 2)
+    xr, yr = (torch.randn(2 * T, D, device=dev, dtype=bf) for _ in range(2))
+    out["block_norm_fwd"] = (lambda: gated_residual_norm(xr, yr, w, gate=w, pre_weight=w), 4 * xr.numel() * 2,
+                             2 * xr.numel() * 2)
+    leaves = [t.clone().requires_grad_() for t in (xr, yr, w, w, w)]
+    h, n = gated_residual_norm(leaves[0], leaves[1], leaves[2], gate=leaves[3], pre_weight=leaves[4])
+    dhn = torch.randn_like(xr)
+    out["block_norm_bwd"] = (lambda: torch.autograd.grad((h, n), leaves, (dhn, dhn), retain_graph=True),
+                             6 * xr.numel() * 2, 4 * xr.numel() * 2)
+    ids = torch.randint(0, V, (T, 64), device=dev)
+    top = torch.randn(T, 64, device=dev)
+    counts, rows_loss = E.distill_count(logits, V, ids, top, tgt, -100), torch.empty(T, device=dev)
+    out["distill_rows"] = (lambda: E.distill_rows_(logits, ids, top, tgt, 2.0, 0.5, -100, counts, rows_loss),
+                           2 * logits.numel() * 2, logits.numel() * 2)
+
     # P2P-style pull-reduce, 8 "ranks" whose buffers are local here (the kernel of the
     # overlapped gradient reduce-scatter): reads 8 x rows, writes 1 x rows
     ws, rows = 8, F * D // 8

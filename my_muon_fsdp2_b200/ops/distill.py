@@ -50,8 +50,8 @@ def _check(rows, device, vocab, teacher_ids, teacher_logits, targets, temperatur
             raise ValueError(f"distillation: {name} must be on the logits' device")
     if vocab < 1:
         raise ValueError("distillation: the vocabulary is empty")
-    if not (math.isfinite(temperature) and temperature > 0):
-        raise ValueError(f"distillation: temperature must be positive and finite, got {temperature}")
+    if not 1e-3 <= temperature <= 1e3:
+        raise ValueError(f"distillation: temperature must be from 1e-3 to 1e3, got {temperature}")
     if not 0 <= alpha <= 1:
         raise ValueError(f"distillation: alpha must be from 0 to 1, got {alpha}")
     if targets is None and alpha != 1:

@@ -180,6 +180,8 @@ def _check(q, k, rot, positions, inplace) -> None:
                 raise RuntimeError("apply_rotary: inplace=True is for tensors outside autograd")
             if x.stride(-1) != 1 or any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
                 raise ValueError("apply_rotary: inplace=True needs contiguous heads in memory of their own")
+        if k is not None and q.numel() and q.data_ptr() == k.data_ptr():
+            raise ValueError("apply_rotary: inplace=True needs q and k in memory of their own")
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotaryEmbedding,
@@ -189,8 +191,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotaryEmbed
     q: [batch, seq, q_heads, head_dim] or [tokens, q_heads, head_dim], k the same with its own number
     of heads; any strides (views of a packed projection need no copy).  ``positions``: int64 or int32,
     broadcast over the leading dimensions (default 0, 1, ... along the sequence; any value, also
-    negative).  ``inplace`` writes into q and k (no gradient): the form for new tokens that go to a
-    cache.  With autograd the results are new contiguous tensors.
+    negative).  ``inplace`` writes into q and k, which must not overlap (no gradient): the form for new
+    tokens that go to a cache.  With autograd the results are new contiguous tensors.
     """
     _check(q, k, rotary, positions, inplace)
     if not q.is_cuda:

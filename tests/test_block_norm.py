@@ -306,3 +306,27 @@ def test_gpu_same_bits_streams_and_graph():
     g.replay()
     want = _run(t, True, 1e-5, 1.0, 1.0)
     assert all(torch.equal(out[k], want[k]) for k in want)
+
+
+@pytest.mark.gpu
+def test_gpu_offsets_past_32_bits():
+    """More than 2^31 values: the last rows are those of a call on them alone."""
+    R, D = 530000, 4096
+    x = torch.empty(R, D, device="cuda", dtype=torch.bfloat16)
+    t = _inputs((3,), D, torch.bfloat16, False, None, True, True, "cuda")
+    x[-3:] = t["x"]
+    w = dict(post_weight=t["post_weight"], pre_weight=t["pre_weight"])
+    want = gated_residual_norm(t["x"], t["x"], **w)
+    got = gated_residual_norm(x, x, **w)
+    assert torch.equal(got[0][-3:], want[0]) and torch.equal(got[1][-3:], want[1])
+    del got
+    small = t["x"].clone().requires_grad_()
+    (wg,) = torch.autograd.grad(gated_residual_norm(small, small, **w), small, (t["dh"], t["dn"]))
+    x[:-3] = 1
+    x.requires_grad_()
+    dh = torch.zeros_like(x)
+    dh[-3:] = t["dh"]
+    dn = torch.zeros_like(x)
+    dn[-3:] = t["dn"]
+    (g,) = torch.autograd.grad(gated_residual_norm(x, x, **w), x, (dh, dn))
+    assert torch.equal(g[-3:], wg) and not g[:-3].any()

@@ -151,7 +151,7 @@ def test_refusals():
     z, ids, a, y = _inputs(4, 9, 3)
     f = distillation_loss
     for bad in (lambda: f(z, ids[:3], a), lambda: f(z, ids, a[:, :2]), lambda: f(z, ids, a, y[:3]), lambda: f(z, ids, a, alpha=0.5),
-                lambda: f(z, ids, a, temperature=0.0), lambda: f(z, ids, a, temperature=math.nan), lambda: f(z, ids, a, y, alpha=1.5),
+                lambda: f(z, ids, a, temperature=0.0), lambda: f(z, ids, a, temperature=math.nan), lambda: f(z, ids, a, temperature=1e4), lambda: f(z, ids, a, y, alpha=1.5),
                 lambda: f(z, ids, a, y, alpha=math.nan), lambda: f(z, ids, a, reduction="sum"), lambda: f(z, ids[:, :0], a[:, :0]),
                 lambda: f(z, ids.repeat(1, 400), a.repeat(1, 400)), lambda: f(z[:, :0], ids, a), lambda: f(z, ids + 9, a),
                 lambda: f(z, ids, a, y.clamp_min(0) + 9, alpha=0.5), lambda: f(z, ids, a.clone().requires_grad_()),
@@ -344,3 +344,23 @@ def test_gpu_fused_linear(N, D, V, chunk):
         assert float((got.double() - ref).norm() / ref.norm()) < rel
     with pytest.raises(RuntimeError, match="second time"):
         torch.autograd.grad(loss, x)
+
+
+@pytest.mark.gpu
+def test_gpu_offsets_past_32_bits():
+    """More than 2^31 logits: the last rows are those of a call on them alone (but for how many blocks share
+    a row there, which orders its sums)."""
+    N, V = 17000, 128256
+    z, ids, a, y = _inputs(5, V, 7, torch.bfloat16, "cuda")
+    big = torch.zeros(N, V, device="cuda", dtype=torch.bfloat16)
+    big[-5:] = z
+    more = lambda t, fill: torch.cat([torch.full((N - 5,) + t.shape[1:], fill, device="cuda", dtype=t.dtype), t])  # noqa: E731
+    args = (more(ids, -1), more(a, 0.0), more(y, -100))
+    for reduction in ("none", "mean"):
+        want = distillation_loss(z.requires_grad_(), ids, a, y, temperature=2.0, alpha=0.5, reduction=reduction)
+        (wg,) = torch.autograd.grad(want.sum(), z)
+        got = distillation_loss(big.requires_grad_(), *args, temperature=2.0, alpha=0.5, reduction=reduction)
+        (g,) = torch.autograd.grad(got.sum(), big)
+        assert torch.allclose(got[-5:] if reduction == "none" else got, want, rtol=1e-5)
+        assert torch.allclose(g[-5:].float(), wg.float(), rtol=2**-7, atol=1e-12) and not g[:-5].any()
+        del g

@@ -140,6 +140,8 @@ def test_refusals():
         apply_rotary(k.expand(1, 2, 3, 8), None, rot, inplace=True)
     with pytest.raises(ValueError):
         apply_rotary(torch.zeros(1, 2, 8, 3).transpose(2, 3), None, rot, inplace=True)
+    with pytest.raises(ValueError):
+        apply_rotary(q, q, rot, inplace=True)
 
 
 # ---------------------------------------------------------------------------------- GPU
@@ -244,3 +246,27 @@ def test_gpu_streams_and_graph():
     q.mul_(2)
     g.replay()
     assert all(torch.equal(x, y) for x, y in zip(out, apply_rotary(q, k, rot, pos)))
+
+
+@pytest.mark.gpu
+def test_gpu_offsets_past_32_bits():
+    """More than 2^31 values: the last tokens are those of a call on them alone."""
+    rot = RotaryEmbedding(128, 500000.0)
+    T = 270000
+    q = torch.empty(1, T, 64, 128, device="cuda", dtype=torch.bfloat16)
+    q[:, -3:] = _rand((1, 3, 64, 128), torch.bfloat16, "cuda")
+    want = apply_rotary(q[:, -3:].clone(), None, rot, torch.arange(T - 3, T, device="cuda"))
+    assert torch.equal(apply_rotary(q, None, rot)[:, -3:], want)
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    rot = RotaryEmbedding(8, interleaved=True)
+    flat = torch.zeros(1 + 2 * 3 * 8, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):  # neighbouring pairs that straddle an access, nowhere to copy them to
+        apply_rotary(flat[1:].view(1, 2, 3, 8), None, rot, inplace=True)
+    with pytest.raises(ValueError):
+        apply_rotary(flat[:-1].view(1, 2, 3, 8), None, rot, torch.arange(2))
+    x = torch.zeros(1, 2, 3, 8, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(apply_rotary(x, None, rot).sum(), x, create_graph=True)
