@@ -18,9 +18,9 @@
 // each thread its own vectors, so that others are on their way while it is at one or two rows' two
 // reductions.  Sums over rows stay in registers, 8 columns a thread (16 for the widest rows), and leave
 // once, as one partial row a worker (one a run for the gate).  A second kernel adds the partials in a fixed
-// order, so that equal calls give equal bits.  8192 x 4096 bf16 with both norms and a gate: 97 us, and 5.5
-// for the sums (403 MB, 64 % of the copy rate); the arithmetic, through packed fp32 instructions, takes
-// about as long as the copies.  One row a turn 102 us; unpacked arithmetic, sums in shared memory and
+// order, so that equal calls give equal bits.  8192 x 4096 bf16 with both norms and a gate: 90 us, and 5.5
+// for the sums (403 MB, 69 % of the copy rate); the arithmetic, through packed fp32 instructions, takes
+// about as long as the copies.  With one row a turn 5 us more; unpacked arithmetic, sums in shared memory and
 // no copies ahead 152; 16 columns a thread and two blocks an SM, weights loaded again for each row, 140.
 #include <algorithm>
 #include <stdexcept>
@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
                                                                         const BwdParts parts, int tpr, int inputs,
                                                                         int stages) {
   constexpr int N = NV * VEC, H = N / 2;
-  // whether y^ and h^ stay in registers from one reduction to the next and the weights from row to row,
-  // or are formed from the copies and loaded again (for 16 columns a thread there is no room)
+  // whether the weights stay in registers from row to row or are loaded again (for 16 columns a thread there
+  // is no room)
   constexpr bool KEEP = N <= 8;
   constexpr int ROWS = kRows<N, LN>;  // in one turn, so that they share its barriers
   extern __shared__ __align__(16) unsigned char smem[];
@@ -73,9 +73,6 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   const T* pb = static_cast<const T*>(a.post_b);
   const T* nw = static_cast<const T*>(a.pre_w);
   const bool gated = a.gate != nullptr, token_gate = gated && a.rows_per_gate == 1;
-  const T* in[INPUTS] = {static_cast<const T*>(nw ? a.dn : nullptr), static_cast<const T*>(a.dh),
-                         static_cast<const T*>(nw ? a.x : nullptr), static_cast<const T*>(pw || gated || nw ? a.y : nullptr),
-                         static_cast<const T*>(token_gate ? a.gate : nullptr)};
   // stage s's vector k of row r's input i is place(s, r)[(i * NV + k) * threads]; what is not copied there
   // is 0
   auto place = [&](int stage, int r) {
@@ -112,14 +109,19 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
         if (ahead.i + r < ahead.rows) {
           const int64_t off = static_cast<int64_t>(ahead.first + ahead.i + r) * cols + g.lane * VEC;
           R* to = place(put, r);
+          auto fetch = [&](int i, const void* from) {
 #pragma unroll
-          for (int i = 0; i < INPUTS; ++i) {
-            if (in[i]) {
-#pragma unroll
-              for (int k = 0; k < NV; ++k)
-                if (col(k) < cols) copy_ahead<T, VEC>(to + (i * NV + k) * threads, in[i] + off + k * tpr * VEC);
-            }
+            for (int k = 0; k < NV; ++k)
+              if (col(k) < cols)
+                copy_ahead<T, VEC>(to + (i * NV + k) * threads, static_cast<const T*>(from) + off + k * tpr * VEC);
+          };
+          if (nw) {
+            fetch(IN_DN, a.dn);
+            fetch(IN_X, a.x);
           }
+          if (a.dh) fetch(IN_DH, a.dh);
+          if (pw || gated || nw) fetch(IN_Y, a.y);
+          if (token_gate) fetch(IN_GATE, a.gate);
         } else {
           clear(put, r);
         }
@@ -249,9 +251,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
       sy[r] = next_y[r];
       sh[r] = next_h[r];
     }
-    Cursor after = now;
-    step(after);
-    load_stats(after, next_y, next_h);
+    {
+      Cursor after = now;
+      step(after);
+      load_stats(after, next_y, next_h);
+    }
     auto load_y = [&](int r, V& u) {  // y^ (y without a post norm)
       input(r, IN_Y, u);
       if (pw) {
@@ -277,13 +281,6 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
         h.p[i] = ffma2(rho, w.p[i], h.p[i]);
         h.p[i] = LN ? ffma2(h.p[i], s, m) : fmul2(h.p[i], s);
       }
-    };
-    auto load_b = [&](int r, V& b) {  // dn w_pre
-      V pre;
-      input(r, IN_DN, b);
-      load_pre(pre);
-#pragma unroll
-      for (int i = 0; i < H; ++i) b.p[i] = fmul2(b.p[i], pre.p[i]);
     };
     constexpr int SUMS = LN ? 2 : 1;
     float t[ROWS * SUMS];
@@ -312,11 +309,6 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
       g.sum(t);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        if constexpr (!KEEP) {
-          load_y(r, u[r]);
-          load_h(r, u[r], h[r]);
-          load_b(r, d[r]);
-        }
         V dh;
         input(r, IN_DH, dh);
         const float k = -sh[r].rstd * inv;
@@ -390,7 +382,6 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         if (pw) {
-          if constexpr (!KEEP) load_y(r, u[r]);
           const float k = -sy[r].rstd * inv;
           const float2 s = both(sy[r].rstd), c2 = both(k * t[r * SUMS]);
 #pragma unroll
@@ -436,7 +427,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
       sum_a.fill(0.f);
       if constexpr (LN) sum_b.fill(0.f);
     }
-    now = after;
+    step(now);
     if (++get == stages) get = 0;
   }
   const int64_t at = static_cast<int64_t>(worker) * cols;
