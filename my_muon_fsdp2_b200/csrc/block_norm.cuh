@@ -12,8 +12,8 @@ namespace mmf {
 
 namespace {
 
-// `tpr` threads of the block that share one row (a power of two from 32 up).  Every thread of the
-// block takes part in every reduction.
+// `tpr` threads of the block that share one row (whole warps).  Every thread of the block takes part in
+// every reduction.
 struct RowGroup {
   int tpr, row, lane, warp0, warps;
   float* red;  // [2][4][32], used in turn so that one barrier a reduction is enough; 16-byte aligned
@@ -51,11 +51,14 @@ struct RowGroup {
 
  private:
   __device__ __forceinline__ float over_warps(const float* r) const {
-    if (warps == 2) return r[0] + r[1];
     float t = 0.f;
-    for (int i = 0; i < warps; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(r + i);
-      t += (v.x + v.y) + (v.z + v.w);
+    if (warps % 4 == 0) {  // then every row's part of r is on a 16-byte boundary
+      for (int i = 0; i < warps; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(r + i);
+        t += (v.x + v.y) + (v.z + v.w);
+      }
+    } else {
+      for (int i = 0; i < warps; ++i) t += r[i];
     }
     return t;
   }
@@ -132,28 +135,28 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // 1 / sqrt(mean square + eps), or with LN the mean and 1 / sqrt(variance + eps), of a row whose values
 // behind its end are 0; inv = 1 / cols.  The variance is taken around the mean in a second reduction: a mean that is large
 // against the deviation cancels nothing.
-template <int VEC, int NV, bool LN>
-__device__ __forceinline__ Stat row_stat(RowGroup& g, const float (&v)[NV][VEC], int cols, float inv, float eps) {
-  float s = 0.f, mean = 0.f;
+template <int N, int VEC, bool LN>
+__device__ __forceinline__ Stat row_stat(RowGroup& g, const Values<N>& v, int cols, float inv, float eps) {
+  float2 s = both(0.f);
+  float mean = 0.f;
   if constexpr (LN) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) mean += v[k][e];
-    mean = g.sum(mean) * inv;
+    for (int i = 0; i < N / 2; ++i) s = fadd2(s, v.p[i]);
+    mean = g.sum(s.x + s.y) * inv;
+    s = both(0.f);
   }
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    if (!LN || (g.lane + k * g.tpr) * VEC < cols) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = v[k][e] - mean;
-        s = fmaf(d, d, s);
-      }
+  for (int i = 0; i < N / 2; ++i) {
+    if constexpr (LN) {
+      // the values behind the row's end are no distance from the mean; a pair is of one vector or (VEC 1) two
+      const bool first = (g.lane + 2 * i / VEC * g.tpr) * VEC < cols, second = (g.lane + (2 * i + 1) / VEC * g.tpr) * VEC < cols;
+      const float2 d = fadd2(v.p[i], both(-mean));
+      s = ffma2(make_float2(first ? d.x : 0.f, second ? d.y : 0.f), d, s);
+    } else {
+      s = ffma2(v.p[i], v.p[i], s);
     }
   }
-  s = g.sum(s);
-  return {rsqrtf(fmaf(s, inv, eps)), mean};
+  return {rsqrtf(fmaf(g.sum(s.x + s.y), inv, eps)), mean};
 }
 
 constexpr int kMaxCols = 8192;
@@ -165,11 +168,7 @@ constexpr int kMaxThreads = 512;
 template <typename T, bool LN, int VEC, typename Go>
 void dispatch_row_width(const Go& go, int cols) {
   constexpr int NV = Go::kValues > VEC ? Go::kValues / VEC : 1;
-  auto threads = [&](int values) {
-    int t = 32;
-    while (t * values < cols) t *= 2;
-    return t;
-  };
+  auto threads = [&](int values) { return ((cols + values - 1) / values + 31) / 32 * 32; };
   if (cols <= kMaxThreads * NV * VEC) return go.template run<T, VEC, NV, LN>(threads(NV * VEC));
   if constexpr (kMaxThreads * NV * VEC < kMaxCols) go.template run<T, VEC, 2 * NV, LN>(threads(2 * NV * VEC));
 }

@@ -491,8 +491,7 @@ struct Backward {
   template <typename T, int VEC, int NV, bool LN>
   void run(int tpr) const {
     auto kernel = block_norm_bwd_kernel<T, VEC, NV, LN>;
-    const int block = tpr < 128 ? 128 : tpr;
-    const int groups = block / tpr;
+    const int groups = tpr < 128 ? 128 / tpr : 1, block = groups * tpr;  // narrow rows: several to a block
     // two rows copied ahead, one or none where they are too wide for that
     const int inputs = a.gate && a.rows_per_gate == 1 ? INPUTS : INPUTS - 1;
     const int stage = kRows<NV * VEC, LN> * inputs * NV * VEC * static_cast<int>(sizeof(T)) * block;
