@@ -427,14 +427,15 @@ Tensor distill_forward(const Tensor& logits, const Tensor& ids, const Tensor& te
     a.grad_ld = grad.stride(0);
   }
   if (stats.defined()) a.stats = stats.data_ptr<float>();
+  Tensor loss = torch::empty({a.rows}, logits.options().dtype(torch::kFloat32));
+  a.loss = loss.data_ptr<float>();
   Tensor counts;
   if (mean) {
     counts = distill_count(logits, a.vocab, ids, teacher, targets, c.ignore_index);
     a.counts = counts.data_ptr<int>();
+    a.behind_count = true;
     if (counts_kept) *counts_kept = counts;
   }
-  Tensor loss = torch::empty({a.rows}, logits.options().dtype(torch::kFloat32));
-  a.loss = loss.data_ptr<float>();
   mmf::distill_rows(a, cur_stream());
   return mean ? distill_sum(loss) : loss;
 }

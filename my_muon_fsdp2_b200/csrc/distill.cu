@@ -478,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 6) distill_rows_kernel(const Distill
   const float4 part = lane % kMaxCluster < blocks ? block_part[lane % kMaxCluster] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
   const Part p = warp_join<MODE, kMaxCluster>(Part{part.x, part.y, part.z}, c_a);
   const bool soft = row_slots.x, hard = target >= 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the counts, where this kernel was let start before them
   const Coefficients k = Coefficients::of<MODE>(sc, a.counts, soft, hard, 1.f);
 
   auto put_loss = [&]() {
@@ -566,6 +567,8 @@ __global__ void __launch_bounds__(kThreads) distill_grad_kernel(const DistillArg
 __global__ void __cluster_dims__(kMaxCluster, 1, 1) __launch_bounds__(1024)
     distill_count_kernel(const DistillArgs a, int* counts, int* err) {
   __shared__ int s[2];
+  // what comes behind may start: it waits for this kernel's end before it looks at the counts
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), lane = threadIdx.x & 31;
   if (threadIdx.x < 2) s[threadIdx.x] = 0;
@@ -585,13 +588,23 @@ __global__ void __cluster_dims__(kMaxCluster, 1, 1) __launch_bounds__(1024)
     const bool first = live && filled(mine, 0);
     targets += look_at(a, y, err) >= 0;
     slots += first;
-    for (unsigned rest = __ballot_sync(0xffffffffu, live && !first); rest; rest &= rest - 1) {
-      const int64_t row = base + __ffs(static_cast<int>(rest)) - 1;
-      bool any = false;
-#pragma unroll 2
-      for (int j = 1 + lane; j < a.top; j += 32) any |= filled(row, j);
-      any = __any_sync(0xffffffffu, any);
-      slots += any && lane == 0;
+    // four rows at a time, their loads on their way together
+    for (unsigned rest = __ballot_sync(0xffffffffu, live && !first); rest;) {
+      int64_t row[4];
+      bool any[4], mine_too[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        mine_too[k] = rest != 0;
+        row[k] = base + (rest ? __ffs(static_cast<int>(rest)) - 1 : 0);
+        rest &= rest - 1;
+        any[k] = false;
+      }
+      for (int j = 1 + lane; j < a.top; j += 32) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any[k] |= mine_too[k] && filled(row[k], j);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) slots += __any_sync(0xffffffffu, any[k]) && lane == 0;
     }
   }
   if (bad) atomicCAS(err, 0, ERR_BAD_ARGUMENT);
@@ -708,12 +721,14 @@ void distill_rows(const DistillArgs& a, cudaStream_t stream) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = attr.val.clusterDim.z = 1;
-    attr.val.clusterDim.y = static_cast<unsigned>(blocks);
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.y = static_cast<unsigned>(blocks);
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.behind_count ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, a, scales(a), each, error_word());
   });
   check("distill_rows");

@@ -400,6 +400,7 @@ struct DistillArgs {
   float tau, alpha;
   int64_t ignore_index;
   bool ids_32, upstream_rows;
+  bool behind_count;  // distill_rows is launched right behind distill_count: it may start before that ends
   DType dtype, teacher_dtype;
 };
 int64_t distill_max_vocab(DType dtype);
