@@ -1,12 +1,16 @@
 // PyTorch bindings of the operators that take bf16, fp16 and fp32 (rotary positions, block norms,
 // distillation).  Their autograd nodes live here rather than in Python: a backward pass then runs
 // without the interpreter, which a small training step would otherwise wait for.
-// Every function checks devices, dtypes and layouts and enqueues on the current stream.
+// Every function checks devices, dtypes, shapes and layouts and enqueues on the current stream.  The
+// checks of a user's call are made here, in 1 us rather than the interpreter's 4 to 6, of which a
+// single token's call would feel every one; what is refused here is named by the Python function's own check.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <string>
 #include <vector>
 
 #include "kernels.h"
@@ -19,6 +23,10 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+// Numbers go into messages as text: where the C++ runtime is linked in statically a stream of the shared
+// libraries' runtime formats none (it faults for want of its locale).
+std::string num(int64_t n) { return std::to_string(n); }
 
 void check_cuda(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), "mmf: ", name, " must be a CUDA tensor");
@@ -151,12 +159,28 @@ class RotaryFn : public torch::autograd::Function<RotaryFn> {
   }
 };
 
-std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const OptTensor& positions, const Tensor& turns,
-                           int64_t rotary_dim, bool interleaved, double magnitude, bool in_place) {
+py::object pair_or_one(const std::vector<Tensor>& out, bool pair) {
+  return pair ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
+}
+
+py::object rotary(const Tensor& q, const OptTensor& k, const OptTensor& positions, const Tensor& turns, int64_t head_dim,
+                  int64_t rotary_dim, bool interleaved, double magnitude, bool in_place) {
+  const bool pair = k.has_value();
+  TORCH_CHECK(q.dim() >= 3 && q.size(-1) == head_dim, "mmf: rotary: q must be [..., heads, ", num(head_dim), "]");
   const OptTensor oq(q);
-  if (!wants_grad({&oq, &k})) return rotary_raw(q, k, positions, turns, rotary_dim, interleaved, magnitude, false, in_place);
-  TORCH_CHECK(!in_place, "mmf: rotary: in place is for tensors outside autograd");
-  return RotaryFn::apply(q, k, positions, turns, rotary_dim, interleaved, magnitude);
+  const bool grad = wants_grad({&oq, &k});
+  if (in_place) {
+    TORCH_CHECK(!grad, "mmf: rotary: in place is for tensors outside autograd");
+    auto own = [](const Tensor& t) {
+      bool ok = t.dim() == 0 || t.stride(-1) == 1;
+      for (int64_t i = 0; i < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) != 0);
+      return ok;
+    };
+    TORCH_CHECK(own(q) && (!pair || own(*k)) && (!pair || q.numel() == 0 || q.data_ptr() != k->data_ptr()),
+                "mmf: rotary: in place needs contiguous heads in memory of their own");
+  }
+  if (!grad) return pair_or_one(rotary_raw(q, k, positions, turns, rotary_dim, interleaved, magnitude, false, in_place), pair);
+  return pair_or_one(RotaryFn::apply(q, k, positions, turns, rotary_dim, interleaved, magnitude), pair);
 }
 
 // ------------------------------------ block norms -----------------------------------------
@@ -169,7 +193,7 @@ struct NormConf {
 void check_like(const OptTensor& t, const Tensor& x, int64_t n, const char* name) {
   if (!t.has_value()) return;
   TORCH_CHECK(t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->is_contiguous() && t->numel() == n,
-              "mmf: block_norm: ", name, " must be contiguous, of x's device and dtype, with ", n, " values");
+              "mmf: block_norm: ", name, " must be contiguous, of x's device and dtype, with ", num(n), " values");
 }
 
 // {h} or {h, n}; stat_y, stat_h: filled where the backward needs them
@@ -212,7 +236,7 @@ variable_list block_norm_raw(const Tensor& x, const Tensor& y, const OptTensor& 
   a.residual_scale = static_cast<float>(c.residual_scale);
   a.branch_scale = static_cast<float>(c.branch_scale);
   a.layer = c.layer;
-  TORCH_CHECK(cols <= 8192, "mmf: block_norm: rows of up to 8192 values are supported, got ", cols);
+  TORCH_CHECK(cols <= 8192, "mmf: block_norm: rows of up to 8192 values are supported, got ", num(cols));
   mmf::block_norm_fwd(a, cur_stream());
   if (n.defined()) return {h, n};
   return {h};
@@ -296,14 +320,44 @@ class BlockNormFn : public torch::autograd::Function<BlockNormFn> {
   }
 };
 
-std::vector<Tensor> block_norm(const Tensor& x, const Tensor& y, const OptTensor& pw, const OptTensor& pb,
-                               const OptTensor& gate, const OptTensor& nw, const OptTensor& nb, int64_t rows_per_gate,
-                               bool layer, double eps, double residual_scale, double branch_scale) {
+// How many consecutive rows of x share a row of the gate: the gate's leading dimensions are x's up to
+// some dimension, and 1 (or missing altogether) from there on.
+int64_t rows_per_gate(const OptTensor& gate, const Tensor& x) {
+  if (!gate.has_value()) return 1;
+  const auto own = gate->sizes(), all = x.sizes();
+  const bool one = own.size() == 1;
+  TORCH_CHECK((one || own.size() == all.size()) && !own.empty() && own.back() == all.back(),
+              "mmf: block_norm: the gate must be [dim] or of x's dimensions");
+  const size_t lead = all.size() - 1;
+  size_t i = one ? 0 : lead;
+  while (i > 0 && own[i - 1] == 1) --i;
+  int64_t shared = 1;
+  for (size_t j = 0; j < lead; ++j) {
+    TORCH_CHECK(j >= i || own[j] == all[j], "mmf: block_norm: the gate's leading dimensions must be x's, then ones");
+    if (j >= i) shared *= all[j];
+  }
+  return std::max<int64_t>(1, shared);
+}
+
+OptTensor dense(const OptTensor& t) { return t.has_value() ? OptTensor(t->contiguous()) : t; }
+
+py::object block_norm(const Tensor& x, const Tensor& y, const OptTensor& pw, const OptTensor& pb, const OptTensor& gate,
+                      const OptTensor& nw, const OptTensor& nb, bool layer, double eps, double residual_scale,
+                      double branch_scale) {
+  TORCH_CHECK(x.dim() >= 1 && x.sizes() == y.sizes(), "mmf: block_norm: x must be [..., dim] and y of its shape");
+  for (const OptTensor* t : {&pw, &pb, &nw, &nb})
+    TORCH_CHECK(!t->has_value() || (*t)->dim() == 1, "mmf: block_norm: weights and biases must be [dim]");
+  TORCH_CHECK(!(pb.has_value() && !(layer && pw.has_value())) && !(nb.has_value() && !(layer && nw.has_value())),
+              "mmf: block_norm: a bias needs its weight and the layer norm");
+  const int64_t shared = rows_per_gate(gate, x);
   const OptTensor ox(x), oy(y);
+  const Tensor xc = x.contiguous(), yc = y.contiguous();
+  const OptTensor pwc = dense(pw), pbc = dense(pb), gc = dense(gate), nwc = dense(nw), nbc = dense(nb);
   if (!wants_grad({&ox, &oy, &pw, &pb, &gate, &nw, &nb}))
-    return block_norm_raw(x, y, pw, pb, gate, nw, nb, {rows_per_gate, layer, eps, residual_scale, branch_scale}, nullptr,
-                          nullptr);
-  return BlockNormFn::apply(x, y, pw, pb, gate, nw, nb, rows_per_gate, layer, eps, residual_scale, branch_scale);
+    return pair_or_one(block_norm_raw(xc, yc, pwc, pbc, gc, nwc, nbc, {shared, layer, eps, residual_scale, branch_scale},
+                                      nullptr, nullptr), nw.has_value());
+  return pair_or_one(BlockNormFn::apply(xc, yc, pwc, pbc, gc, nwc, nbc, shared, layer, eps, residual_scale, branch_scale),
+                     nw.has_value());
 }
 
 // ------------------------------------ distillation ----------------------------------------
@@ -323,11 +377,11 @@ mmf::DistillArgs distill_args(const Tensor& like, int64_t rows, int64_t vocab, c
               "mmf: distill: ids must be contiguous int64 or int32 [rows, top] on the logits' device");
   TORCH_CHECK(teacher.device() == like.device() && teacher.is_contiguous() && teacher.sizes() == ids.sizes(),
               "mmf: distill: the teacher's logits must be contiguous, of the ids' shape, on the logits' device");
-  TORCH_CHECK(ids.size(1) >= 1 && ids.size(1) <= mmf::distill_max_top(), "mmf: distill: 1 to ", mmf::distill_max_top(),
+  TORCH_CHECK(ids.size(1) >= 1 && ids.size(1) <= mmf::distill_max_top(), "mmf: distill: 1 to ", num(mmf::distill_max_top()),
               " slots a row are supported");
   a.dtype = dtype_of(like, "logits");
   TORCH_CHECK(vocab >= 1 && vocab <= mmf::distill_max_vocab(a.dtype), "mmf: distill: a vocabulary of up to ",
-              mmf::distill_max_vocab(a.dtype), " values of this dtype is supported");
+              num(mmf::distill_max_vocab(a.dtype)), " values of this dtype is supported");
   if (targets.has_value())
     TORCH_CHECK(targets->device() == like.device() && targets->scalar_type() == torch::kInt64 &&
                     targets->is_contiguous() && targets->numel() == rows,
@@ -347,7 +401,7 @@ mmf::DistillArgs distill_args(const Tensor& like, int64_t rows, int64_t vocab, c
 }
 
 void put_logits(mmf::DistillArgs& a, const Tensor& logits) {
-  TORCH_CHECK(logits.dim() == 2 && (logits.numel() == 0 || logits.stride(1) == 1),
+  TORCH_CHECK(logits.dim() == 2 && (logits.numel() == 0 || logits.size(1) == 1 || logits.stride(1) == 1),
               "mmf: distill: logits must be [rows, vocab] with unit column stride");
   a.logits = logits.data_ptr();
   a.ld = logits.size(0) > 1 ? logits.stride(0) : 0;
@@ -498,12 +552,34 @@ class DistillFn : public torch::autograd::Function<DistillFn> {
   }
 };
 
+// logits [..., vocab], ids and teacher [..., top], targets [...]
 Tensor distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const OptTensor& targets, double tau,
                double alpha, int64_t ignore_index, bool mean) {
-  const OptTensor ol(logits);
-  if (wants_grad({&ol})) return DistillFn::apply(logits, ids, teacher, targets, tau, alpha, ignore_index, mean);
-  const c10::cuda::CUDAGuard guard(logits.device());
-  return distill_forward(logits, ids, teacher, targets, {tau, alpha, ignore_index}, mean, Tensor(), Tensor());
+  const int64_t lead = logits.dim() - 1;
+  TORCH_CHECK(lead >= 0 && ids.dim() == lead + 1 && ids.sizes().slice(0, lead) == logits.sizes().slice(0, lead) &&
+                  teacher.sizes() == ids.sizes() && (!targets.has_value() || targets->sizes() == logits.sizes().slice(0, lead)),
+              "mmf: distill: the teacher's slots and the targets must have the logits' leading dimensions");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && teacher.requires_grad()), "mmf: distill: the teacher takes no gradient");
+  TORCH_CHECK(tau >= 1e-3 && tau <= 1e3 && alpha >= 0 && alpha <= 1 && (alpha == 1 || targets.has_value()),
+              "mmf: distill: temperature, alpha or targets out of range");
+  const int64_t vocab = logits.size(-1), top = ids.size(-1);
+  TORCH_CHECK(vocab >= 1 && top >= 1, "mmf: distill: an empty vocabulary, or no slot");
+  int64_t rows = 1;
+  for (int64_t i = 0; i < lead; ++i) rows *= logits.size(i);
+  Tensor z = lead == 1 ? logits : logits.reshape({rows, vocab});
+  if (z.stride(1) != 1 && vocab > 1) z = z.contiguous();
+  const Tensor i = (lead == 1 ? ids : ids.reshape({rows, top})).contiguous();
+  const Tensor t = (lead == 1 ? teacher : teacher.reshape({rows, top})).contiguous();
+  const OptTensor y = targets.has_value() ? OptTensor((lead == 1 ? *targets : targets->reshape({rows})).contiguous()) : targets;
+  const OptTensor ol(z);
+  Tensor loss;
+  if (wants_grad({&ol})) {
+    loss = DistillFn::apply(z, i, t, y, tau, alpha, ignore_index, mean);
+  } else {
+    const c10::cuda::CUDAGuard guard(z.device());
+    loss = distill_forward(z, i, t, y, {tau, alpha, ignore_index}, mean, Tensor(), Tensor());
+  }
+  return mean || lead == 1 ? loss : loss.reshape(logits.sizes().slice(0, lead));
 }
 
 }  // namespace

@@ -20,22 +20,18 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 MAX_DIM = 8192
 
 
-def _rows_per_gate(gate: torch.Tensor, x: torch.Tensor) -> int:
-    """How many consecutive rows of x share a row of the gate: the gate's leading dimensions are x's
-    up to some dimension, and 1 (or missing altogether) from there on."""
+def _check_gate(gate: torch.Tensor, x: torch.Tensor) -> None:
+    """The gate's leading dimensions are x's up to some dimension, and 1 (or missing altogether) from there on."""
     lead, own = x.shape[:-1], gate.shape[:-1]
     if gate.shape[-1:] == x.shape[-1:]:
         if not own:
-            own = (1,) * len(lead)
+            return
         if len(own) == len(lead):
             i = len(lead)
             while i > 0 and own[i - 1] == 1:
                 i -= 1
             if own[:i] == lead[:i]:
-                shared = 1
-                for n in lead[i:]:
-                    shared *= n
-                return max(1, shared)
+                return
     raise ValueError(f"gated_residual_norm: gate {tuple(gate.shape)} must be [dim], or x's shape {tuple(x.shape)} with "
                      f"ones in the place of trailing leading dimensions (one gate for each sequence: [batch, 1, dim])")
 
@@ -63,6 +59,8 @@ def _check(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, norm) -> No
     for name, b, w in (("post_bias", post_bias, post_weight), ("pre_bias", pre_bias, pre_weight)):
         if b is not None and (w is None or norm != "layer"):
             raise ValueError(f"gated_residual_norm: {name} needs its weight and norm='layer'")
+    if gate is not None:
+        _check_gate(gate, x)
 
 
 def _norm_torch(v, w, b, layer, eps):
@@ -82,14 +80,15 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[
     ``norm``: ``"rms"`` or ``"layer"``, with biases for the latter.  Statistics and sums are fp32, each
     output is rounded once, n is formed from h before its rounding.  Gradients flow to every tensor.
     """
+    if x.is_cuda and norm in ("rms", "layer"):
+        try:
+            return ext().block_norm(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, norm == "layer", eps,
+                                    residual_scale, branch_scale)
+        except (RuntimeError, TypeError):
+            _check(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, norm)  # names what was refused
+            raise
     _check(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, norm)
     layer = norm == "layer"
-    rows_per_gate = _rows_per_gate(gate, x) if gate is not None else 1
-    if x.is_cuda:
-        out = ext().block_norm(x.contiguous(), y.contiguous(), _dense(post_weight), _dense(post_bias), _dense(gate),
-                               _dense(pre_weight), _dense(pre_bias), rows_per_gate, layer, eps, residual_scale,
-                               branch_scale)
-        return tuple(out) if pre_weight is not None else out[0]
     ct = torch.promote_types(x.dtype, torch.float32)
     up = lambda t: None if t is None else t.to(ct)  # noqa: E731
     p = up(y)
@@ -102,6 +101,3 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[
         return h.to(x.dtype)
     return h.to(x.dtype), _norm_torch(h, up(pre_weight), up(pre_bias), layer, eps).to(x.dtype)
 
-
-def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.contiguous()

@@ -101,6 +101,20 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     ``reduction="mean"`` on bf16 and fp32 the gradient is formed together with the loss and kept for
     one backward pass.
     """
+    if logits.is_cuda and reduction in ("mean", "none"):
+        try:
+            return ext().distill(logits, teacher_ids, teacher_logits, targets, temperature, alpha, ignore_index,
+                                 reduction == "mean")
+        except (RuntimeError, TypeError):
+            _flat(logits, teacher_ids, teacher_logits, targets, temperature, alpha, reduction)  # names what was refused
+            raise
+    z, ids, a, y = _flat(logits, teacher_ids, teacher_logits, targets, temperature, alpha, reduction)
+    loss = _loss_torch(z, ids, a, y, temperature, alpha, ignore_index, reduction == "mean")
+    return loss.reshape(logits.shape[:-1]) if reduction == "none" else loss
+
+
+def _flat(logits, teacher_ids, teacher_logits, targets, temperature, alpha, reduction):
+    """The arguments, looked over, with one leading dimension."""
     if reduction not in ("mean", "none"):
         raise ValueError(f"distillation: reduction must be 'mean' or 'none', got {reduction!r}")
     if logits.dim() < 1:
@@ -111,22 +125,15 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     if teacher_ids.shape[:-1] != lead or (targets is not None and targets.shape != lead):
         raise ValueError(f"distillation: teacher_ids {tuple(teacher_ids.shape)} and targets must have the logits' "
                          f"leading dimensions {tuple(lead)}")
-    V = logits.shape[-1]
-    z = logits if logits.dim() == 2 else logits.reshape(-1, V) if V else logits.new_empty(lead.numel(), 0)
-    ids = teacher_ids if teacher_ids.dim() == 2 else teacher_ids.reshape(z.shape[0], teacher_ids.shape[-1])
     if teacher_logits.shape != teacher_ids.shape:
         raise ValueError("distillation: teacher_logits must have the shape of teacher_ids")
-    a = teacher_logits if teacher_logits.dim() == 2 else teacher_logits.reshape(ids.shape)
-    y = targets if targets is None or targets.dim() == 1 else targets.reshape(-1)
-    _check(z.shape[0], z.device, V, ids, a, y, temperature, alpha)
-    if z.is_cuda:
-        if z.stride(1) != 1 and V > 1:
-            z = z.contiguous()
-        loss = ext().distill(z, ids.contiguous(), a.contiguous(), None if y is None else y.contiguous(), temperature,
-                             alpha, ignore_index, reduction == "mean")
-    else:
-        loss = _loss_torch(z, ids, a, y, temperature, alpha, ignore_index, reduction == "mean")
-    return loss.reshape(lead) if reduction == "none" and logits.dim() != 2 else loss
+    V, rows = logits.shape[-1], lead.numel()
+    z = logits.reshape(rows, V)
+    ids = teacher_ids.reshape(rows, teacher_ids.shape[-1])
+    a = teacher_logits.reshape(ids.shape)
+    y = None if targets is None else targets.reshape(-1)
+    _check(rows, z.device, V, ids, a, y, temperature, alpha)
+    return z, ids, a, y
 
 
 class _LinearDistillFn(torch.autograd.Function):

@@ -194,14 +194,17 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotaryEmbed
     negative).  ``inplace`` writes into q and k, which must not overlap (no gradient): the form for new
     tokens that go to a cache.  With autograd the results are new contiguous tensors.
     """
+    if isinstance(q, torch.Tensor) and q.is_cuda and isinstance(rotary, RotaryEmbedding):
+        try:
+            return ext().rotary(q, k, positions, rotary._table(q.device), rotary.head_dim, rotary.rotary_dim,
+                                rotary.interleaved, rotary.magnitude, inplace)
+        except (RuntimeError, TypeError):
+            _check(q, k, rotary, positions, inplace)  # names what was refused
+            raise
     _check(q, k, rotary, positions, inplace)
-    if not q.is_cuda:
-        pos = torch.arange(q.shape[-3], device=q.device) if positions is None else positions
-        cos, sin = rotary.cos_sin(pos, torch.float64 if q.dtype == torch.float64 else torch.float32)
-        out = [_rotate_torch(x, cos, sin, rotary) for x in (q, k) if x is not None]
-        if inplace:
-            out = [x.copy_(o) for x, o in zip((q, k), out)]
-        return tuple(out) if k is not None else out[0]
-    out = ext().rotary(q, k, positions, rotary._table(q.device), rotary.rotary_dim, rotary.interleaved,
-                       rotary.magnitude, inplace)
+    pos = torch.arange(q.shape[-3], device=q.device) if positions is None else positions
+    cos, sin = rotary.cos_sin(pos, torch.float64 if q.dtype == torch.float64 else torch.float32)
+    out = [_rotate_torch(x, cos, sin, rotary) for x in (q, k) if x is not None]
+    if inplace:
+        out = [x.copy_(o) for x, o in zip((q, k), out)]
     return tuple(out) if k is not None else out[0]

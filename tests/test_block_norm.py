@@ -330,3 +330,22 @@ def test_gpu_offsets_past_32_bits():
     dn[-3:] = t["dn"]
     (g,) = torch.autograd.grad(gated_residual_norm(x, x, **w), x, (dh, dn))
     assert torch.equal(g[-3:], wg) and not g[:-3].any()
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    """What the CPU form refuses the kernels' entry refuses in the same way."""
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, device="cuda", dtype=dtype)  # noqa: E731
+    x, w, f = z(2, 3, 8), torch.ones(8, device="cuda"), gated_residual_norm
+    for bad in (lambda: f(x, x[:1]), lambda: f(x, x.view(3, 2, 8)), lambda: f(x, x, w[:4]), lambda: f(x, x, w.view(1, 8)),
+                lambda: f(x, x, gate=x[:, :2]), lambda: f(x, x, gate=z(1, 3, 8)), lambda: f(x, x, gate=z(2, 8)),
+                lambda: f(x, x, gate=z(2, 3, 1)), lambda: f(x, x, gate=z(1, 2, 3, 8)), lambda: f(x, x, gate=z()),
+                lambda: f(x, x, norm="group"), lambda: f(x, x, w, w), lambda: f(x, x, None, w, norm="layer"),
+                lambda: f(x, x, pre_bias=w, norm="layer"), lambda: f(x, x, pre_weight=w, pre_bias=w),
+                lambda: f(z(2, 0), z(2, 0)), lambda: f(z(), z()), lambda: f(z(), z(), gate=z()), lambda: f(z(1, 8193), z(1, 8193))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: f(x, x.bfloat16()), lambda: f(x, x, w.half()), lambda: f(x.long(), x.long()), lambda: f(x, x, gate=w.double()),
+                lambda: f(x.double(), x.double()), lambda: f(x, x.cpu()), lambda: f(x, x, w.cpu())):
+        with pytest.raises(TypeError):
+            bad()

@@ -364,3 +364,41 @@ def test_gpu_offsets_past_32_bits():
         assert torch.allclose(got[-5:] if reduction == "none" else got, want, rtol=1e-5)
         assert torch.allclose(g[-5:].float(), wg.float(), rtol=2**-7, atol=1e-12) and not g[:-5].any()
         del g
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    """What the CPU form refuses before it looks at values the kernels' entry refuses in the same way."""
+    z, ids, a, y = _inputs(4, 9, 3, torch.float32, "cuda")
+    f = distillation_loss
+    for bad in (lambda: f(z, ids[:3], a), lambda: f(z, ids, a[:, :2]), lambda: f(z, ids, a, y[:3]), lambda: f(z, ids, a, alpha=0.5),
+                lambda: f(z, ids, a, temperature=0.0), lambda: f(z, ids, a, temperature=math.nan), lambda: f(z, ids, a, temperature=1e4),
+                lambda: f(z, ids, a, y, alpha=1.5), lambda: f(z, ids, a, y, alpha=math.nan), lambda: f(z, ids, a, reduction="sum"),
+                lambda: f(z, ids[:, :0], a[:, :0]), lambda: f(z, ids.repeat(1, 400), a.repeat(1, 400)), lambda: f(z[:, :0], ids, a),
+                lambda: f(z, ids, a.clone().requires_grad_()), lambda: f(z.view(2, 2, 9), ids, a), lambda: f(z.sum(), ids, a),
+                lambda: f(z, ids.cpu(), a), lambda: f(z, ids, a.cpu()), lambda: f(z, ids, a, y.cpu(), alpha=0.5)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: f(z.long(), ids, a), lambda: f(z.double(), ids, a), lambda: f(z, ids.float(), a), lambda: f(z, ids, a.long()),
+                lambda: f(z, ids, a, y.int(), alpha=0.5)):
+        with pytest.raises(TypeError):
+            bad()
+
+
+@pytest.mark.gpu
+def test_gpu_one_word_and_more_dimensions():
+    """A vocabulary of one word whose column stride means nothing, and leading dimensions that are views."""
+    z = torch.randn(5, 4, device="cuda")[:, 1:2].as_strided((5, 1), (4, 3), 1)
+    one = torch.zeros(5, 1, dtype=torch.long, device="cuda")
+    # lse - z: R = fl(z / ln 2) and its product with ln 2 round by 2^-24 |z| each, besides the error of exp and log
+    assert abs(distillation_loss(z, one, torch.zeros(5, 1, device="cuda")).item()) <= LSE + 2**-23 * z.abs().max().item()
+    z, ids, a, y = _inputs(12, 300, 4, torch.float32, "cuda")
+    flat = distillation_loss(z, ids, a, y, alpha=0.5, reduction="none")
+    lead = lambda t: t.view(3, 4, *t.shape[1:])  # noqa: E731
+    zl = lead(z).transpose(0, 1).requires_grad_()
+    got = distillation_loss(zl, lead(ids).transpose(0, 1), lead(a).transpose(0, 1), lead(y).t(), alpha=0.5, reduction="none")
+    assert got.shape == (4, 3) and torch.equal(got.t().reshape(12), flat)
+    (g,) = torch.autograd.grad(got.sum(), zl)
+    zf = z.detach().requires_grad_()
+    (want,) = torch.autograd.grad(distillation_loss(zf, ids, a, y, alpha=0.5, reduction="none").sum(), zf)
+    assert torch.equal(g.transpose(0, 1).reshape(12, 300), want)

@@ -144,6 +144,17 @@ def test_refusals():
         apply_rotary(q, q, rot, inplace=True)
 
 
+def test_messages_of_the_entry_hold_numbers():
+    """A refusal that names a number comes back as an error (its text is formed in the extension)."""
+    from my_muon_fsdp2_b200._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    q = torch.zeros(4, 2, 9)
+    with pytest.raises(RuntimeError, match=r"heads, 8\]"):
+        ext().rotary(q, None, None, q, 8, 8, False, 1.0, False)
+
+
 # ---------------------------------------------------------------------------------- GPU
 # (batch, seq, q heads, k heads, head_dim, rotary_dim): one token, odd lengths, heads that are no
 # multiple of what a thread takes, parts whose width allows 16-, 4- and 2-byte accesses only
@@ -270,3 +281,25 @@ def test_gpu_refusals():
     x = torch.zeros(1, 2, 3, 8, device="cuda", requires_grad=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(apply_rotary(x, None, rot).sum(), x, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_gpu_refusals_of_arguments():
+    """What the CPU form refuses the kernel's entry refuses in the same way."""
+    rot = RotaryEmbedding(8)
+    q, k = torch.zeros(1, 2, 3, 8, device="cuda"), torch.zeros(1, 2, 1, 8, device="cuda")
+    pos = lambda *s: torch.zeros(s, dtype=torch.long, device="cuda")  # noqa: E731
+    for bad in (lambda: apply_rotary(q, k, None), lambda: apply_rotary(q.long(), None, rot), lambda: apply_rotary(q.double(), None, rot),
+                lambda: apply_rotary(q, k, rot, pos(2).float())):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: apply_rotary(q[0, 0], None, rot), lambda: apply_rotary(q[None], None, rot), lambda: apply_rotary(q[..., :6], None, rot),
+                lambda: apply_rotary(q, k[:, :1], rot), lambda: apply_rotary(q, k.bfloat16(), rot), lambda: apply_rotary(q, k.cpu(), rot),
+                lambda: apply_rotary(q, "k", rot),
+                lambda: apply_rotary(q, k, rot, pos(3)), lambda: apply_rotary(q, k, rot, pos(1, 1, 2)), lambda: apply_rotary(q, k, rot, pos()),
+                lambda: apply_rotary(k.expand(1, 2, 3, 8), None, rot, inplace=True), lambda: apply_rotary(q, q, rot, inplace=True),
+                lambda: apply_rotary(torch.zeros(1, 2, 8, 3, device="cuda").transpose(2, 3), None, rot, inplace=True)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        apply_rotary(q.clone().requires_grad_(), k, rot, inplace=True)
