@@ -684,10 +684,29 @@ void typed_mode(const DistillArgs& a, const Go& go) {
   });
 }
 
-constexpr int kSliceGoal = 32 << 10;  // bytes: six blocks an SM
+constexpr int kInFlight = 180 << 10;  // bytes of rows on an SM at once
 constexpr int kSliceMost = 200 << 10;
 constexpr int kSliceLeast = 8 << 10;
 int slot_bytes(int top) { return ((top + 3) & ~3) * 16; }
+
+// Blocks for a row of `bytes`.  What an SM gets through goes by the bytes that it holds at once (a block
+// takes about as long with 64 KB as with 32): the most blocks, hence the smallest slices, that still
+// hold kInFlight of an SM's 228 KB, and where no number of blocks does, the number that holds most.
+int blocks_of_row(int64_t bytes, int slots) {
+  int best = 1;
+  int64_t most = 0;
+  for (int b = kMaxCluster; b >= 1; --b) {
+    const int64_t slice = bytes / b;
+    if (slice > kSliceMost) break;
+    const int64_t held = slice * std::min<int64_t>(6, (228 << 10) / (slice + slots + 2048));  // 2 KB: a block's own
+    if (held >= kInFlight) return b;
+    if (held > most) {
+      most = held;
+      best = b;
+    }
+  }
+  return best;
+}
 
 }  // namespace
 
@@ -706,11 +725,8 @@ void distill_rows(const DistillArgs& a, cudaStream_t stream) {
   typed_mode(a, [&](auto tag, auto mode) {
     using T = decltype(tag);
     const int64_t bytes = static_cast<int64_t>(a.vocab) * sizeof(T);
-    // blocks a row: slices that fit six to an SM; with few rows more, down to 8 KB each, so that
-    // every SM has one
-    int blocks = 1;
-    while (blocks < kMaxCluster && bytes / blocks > kSliceGoal) blocks *= 2;
-    while (blocks < kMaxCluster && a.rows * blocks < 148 && bytes / blocks > kSliceLeast) blocks *= 2;
+    int blocks = blocks_of_row(bytes, slot_bytes(a.top));
+    while (blocks < kMaxCluster && a.rows * blocks < 148 && bytes / blocks > kSliceLeast) ++blocks;
     if (a.rows > 0x7fffffff) throw std::runtime_error("mmf: distill: too many rows");
     const int each = (a.vocab / Vec<T>::N + blocks - 1) / blocks;
     const int smem = each * 16 + slot_bytes(a.top);
