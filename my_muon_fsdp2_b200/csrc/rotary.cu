@@ -171,7 +171,8 @@ void launch(const RotaryArgs& a, cudaStream_t stream) {
   const int64_t blocks = (tokens + block_tokens - 1) / block_tokens;
   if (tokens > 0x7fffffff) throw std::runtime_error("mmf: rotary: too many tokens");
   const size_t smem = static_cast<size_t>(block_tokens) * half * 2 * sizeof(float);
-  // few tokens: the heads are split over blocks too, each computing the angles for itself
+  // few tokens: the heads are split over blocks too, each computing the angles for itself (1 token of
+  // 40 heads x 128: 2.1 us, 5.1 unsplit; 128 tokens 3.2, 6.4 unsplit)
   int splits = 1;
   while (blocks * splits < 148 && lanes * splits < heads) splits *= 2;
   rotary_kernel<T, VEC, INTERLEAVED>

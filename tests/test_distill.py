@@ -402,3 +402,24 @@ def test_gpu_one_word_and_more_dimensions():
     zf = z.detach().requires_grad_()
     (want,) = torch.autograd.grad(distillation_loss(zf, ids, a, y, alpha=0.5, reduction="none").sum(), zf)
     assert torch.equal(g.transpose(0, 1).reshape(12, 300), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,V,K", [(7, 40, 700), (4, 30001, 1000), (160, 50257, 130), (150, 20003, 257)], ids=str)
+def test_gpu_many_slots_of_few_words(N, V, K, dtype):
+    """Words that come up many times, in one block's slice and over several warps' slots; each number of
+    blocks a row.  Equal calls give equal bits."""
+    z, ids, a, y = _inputs(N, V, K, dtype, "cuda")
+    some = torch.randint(0, V, (30,), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    ids = torch.where(ids >= 0, some[ids % 30], -1)
+    y = torch.where(y >= 0, some[y % 30], y)
+    for reduction in ("mean", "none"):
+        _check(z, ids, a, y, 2.0, 0.5, reduction, 1024.0 if dtype == torch.float16 else 1.0)
+        z.requires_grad_()
+        runs = []
+        for _ in range(3):
+            loss = distillation_loss(z, ids, a, y, alpha=0.5, reduction=reduction)
+            runs.append((loss.detach(), *torch.autograd.grad(loss.sum(), z)))
+        z = z.detach()
+        assert all(torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1]) for r in runs)
