@@ -178,6 +178,9 @@ py::object rotary(const Tensor& q, const OptTensor& k, const OptTensor& position
     };
     TORCH_CHECK(own(q) && (!pair || own(*k)) && (!pair || q.numel() == 0 || q.data_ptr() != k->data_ptr()),
                 "mmf: rotary: in place needs contiguous heads in memory of their own");
+    // a backward pass that kept q or k has to see that they have changed
+    if (!q.is_inference()) q.unsafeGetTensorImpl()->bump_version();
+    if (pair && !k->is_inference()) k->unsafeGetTensorImpl()->bump_version();
   }
   if (!grad) return pair_or_one(rotary_raw(q, k, positions, turns, rotary_dim, interleaved, magnitude, false, in_place), pair);
   return pair_or_one(RotaryFn::apply(q, k, positions, turns, rotary_dim, interleaved, magnitude), pair);

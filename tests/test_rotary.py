@@ -303,3 +303,20 @@ def test_gpu_refusals_of_arguments():
             bad()
     with pytest.raises(RuntimeError):
         apply_rotary(q.clone().requires_grad_(), k, rot, inplace=True)
+
+
+@pytest.mark.gpu
+def test_gpu_inplace_is_seen_by_autograd():
+    """A product that kept q for its backward notices that q was rotated in place."""
+    rot = RotaryEmbedding(8).to("cuda")
+    for mode in ("q", "k"):
+        q, k = torch.randn(1, 2, 3, 8, device="cuda"), torch.randn(1, 2, 1, 8, device="cuda")
+        w = torch.randn(8, 4, device="cuda", requires_grad=True)
+        out = ((q if mode == "q" else k) @ w).sum()
+        apply_rotary(q, k, rot, inplace=True)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(out, w)
+    with torch.inference_mode():
+        q = torch.randn(1, 2, 3, 8, device="cuda")
+        want = apply_rotary(q, None, rot)
+        assert apply_rotary(q, None, rot, inplace=True) is q and torch.equal(q, want)
