@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_fwd_kernel(const Block
 }
 
 struct Forward {
-  static constexpr int kValues = 16;  // a thread, while the row needs no more than kMaxThreads
+  static constexpr int kValues = 16;  // a thread: kMaxThreads take the widest row
   const BlockNormArgs& a;
   cudaStream_t stream;
   template <typename T, int VEC, int NV, bool LN>

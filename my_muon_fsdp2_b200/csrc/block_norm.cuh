@@ -162,15 +162,18 @@ __device__ __forceinline__ Stat row_stat(RowGroup& g, const Values<N>& v, int co
 constexpr int kMaxCols = 8192;
 constexpr int kMaxThreads = 512;
 
+// The columns of the first of two blocks that share a row.
+__host__ __device__ __forceinline__ int first_half(int cols, int vec) { return (cols + 2 * vec - 1) / (2 * vec) * vec; }
+
 // Calls go.run<T, VEC, NV, LN>(threads a row) for the widest access that divides the rows' width and
-// their starts (16 bytes, else 4, else one value), with Go::kValues values a thread (VEC at least), or
-// twice as many where kMaxThreads threads are too few for that.
+// their starts (16 bytes, else 4, else one value), with Go::kValues values a thread (VEC at least); where
+// kMaxThreads threads are too few for that, go.run<T, VEC, NV, LN, true>(threads of half a row).
 template <typename T, bool LN, int VEC, typename Go>
 void dispatch_row_width(const Go& go, int cols) {
   constexpr int NV = Go::kValues > VEC ? Go::kValues / VEC : 1;
-  auto threads = [&](int values) { return ((cols + values - 1) / values + 31) / 32 * 32; };
-  if (cols <= kMaxThreads * NV * VEC) return go.template run<T, VEC, NV, LN>(threads(NV * VEC));
-  if constexpr (kMaxThreads * NV * VEC < kMaxCols) go.template run<T, VEC, 2 * NV, LN>(threads(2 * NV * VEC));
+  auto threads = [&](int n) { return ((n + NV * VEC - 1) / (NV * VEC) + 31) / 32 * 32; };
+  if (cols <= kMaxThreads * NV * VEC) return go.template run<T, VEC, NV, LN>(threads(cols));
+  if constexpr (kMaxThreads * NV * VEC < kMaxCols) go.template run<T, VEC, NV, LN, true>(threads(first_half(cols, VEC)));
 }
 template <typename T, bool LN, typename Go>
 void dispatch_row_vec(const Go& go, const void* const* rows, int n, int cols) {

@@ -16,12 +16,15 @@
 // Bound by memory: dh, dn, x and y are read once, dx and dy written once.  A worker (a group of
 // threads that shares a row) walks over a run of rows, whose data are copied ahead into shared memory,
 // each thread its own vectors, so that others are on their way while it is at one or two rows' two
-// reductions.  Sums over rows stay in registers, 8 columns a thread (16 for the widest rows), and leave
-// once, as one partial row a worker (one a run for the gate).  A second kernel adds the partials in a fixed
-// order, so that equal calls give equal bits.  8192 x 4096 bf16 with both norms and a gate: 90 us, and 5.5
-// for the sums (403 MB, 69 % of the copy rate); the arithmetic, through packed fp32 instructions, takes
-// about as long as the copies.  With one row a turn 5 us more; unpacked arithmetic, sums in shared memory and
-// no copies ahead 152; 16 columns a thread and two blocks an SM, weights loaded again for each row, 140.
+// reductions.  Sums over rows stay in registers, 8 columns a thread, and leave once, as one partial row a
+// worker (one a run for the gate).  Rows of more than 8 x 512 columns are shared by two blocks of a
+// cluster, which exchange the sums of their halves: 8192 x 8192 bf16 240 us (gate for each token 287),
+// where one block with 16 columns a thread had no registers left for the weights, 330 (303).  A second
+// kernel adds the partials in a fixed order, so that equal calls give equal bits.  8192 x 4096 bf16 with
+// both norms and a gate: 90 us, and 5.5 for the sums (403 MB, 69 % of the copy rate); the arithmetic,
+// through packed fp32 instructions, takes about as long as the copies.  With one row a turn 5 us more;
+// unpacked arithmetic, sums in shared memory and no copies ahead 152; 16 columns a thread and two blocks
+// an SM, weights loaded again for each row, 140.
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -49,18 +52,24 @@ struct BwdParts {
 enum { IN_DN, IN_DH, IN_X, IN_Y, IN_GATE, INPUTS };
 
 // Rows that a worker takes in one turn (with a layer norm's sums there is no room for two).
-template <int N, bool LN>
-constexpr int kRows = N <= 8 && !LN ? 2 : 1;
+template <bool LN>
+constexpr int kRows = LN ? 1 : 2;
 
-template <typename T, int VEC, int NV, bool LN>
+// What two blocks that share a row tell one another: the sums of their halves, an asynchronous store that
+// counts its bytes on the receiver's barrier.  Two places in turn: a block that is one reduction ahead
+// has this one's part of that reduction, which this block sends when all its threads have read the last.
+struct PairNotes {
+  float4 part[2];
+  uint64_t bar[2];
+};
+
+// PAIR: a cluster of two blocks shares each row, half the columns each.
+template <typename T, int VEC, int NV, bool LN, bool PAIR>
 __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const BlockNormBwdArgs a, const Plan plan,
                                                                         const BwdParts parts, int tpr, int inputs,
-                                                                        int stages) {
+                                                                        int stages, int* err) {
   constexpr int N = NV * VEC, H = N / 2;
-  // whether the weights stay in registers from row to row or are loaded again (for 16 columns a thread there
-  // is no room)
-  constexpr bool KEEP = N <= 8;
-  constexpr int ROWS = kRows<N, LN>;  // in one turn, so that they share its barriers
+  constexpr int ROWS = kRows<LN>;  // in one turn, so that they share its barriers
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ __align__(16) float red[2 * 4 * 32];
   using R = Raw<T, VEC>;
@@ -68,7 +77,42 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   RowGroup g(tpr, red);
   const int cols = a.cols, threads = static_cast<int>(blockDim.x);
   const int groups = threads / tpr;
-  const int worker = static_cast<int>(blockIdx.x) * groups + g.row, workers = static_cast<int>(gridDim.x) * groups;
+  const int rank = PAIR ? static_cast<int>(blockIdx.x) & 1 : 0;
+  const int worker = PAIR ? static_cast<int>(blockIdx.x) >> 1 : static_cast<int>(blockIdx.x) * groups + g.row;
+  const int workers = PAIR ? static_cast<int>(gridDim.x) >> 1 : static_cast<int>(gridDim.x) * groups;
+  // the block's columns
+  const int base = rank ? first_half(cols, VEC) : 0, end = PAIR && !rank ? first_half(cols, VEC) : cols;
+  __shared__ PairNotes notes;
+  [[maybe_unused]] uint32_t reductions = 0;
+  if constexpr (PAIR) {
+    if (threadIdx.x == 0) {
+      mbar_init(&notes.bar[0], 1);
+      mbar_init(&notes.bar[1], 1);
+      fence_mbar_init();
+      mbar_arrive_expect_tx(&notes.bar[0], sizeof(float4));
+      mbar_arrive_expect_tx(&notes.bar[1], sizeof(float4));
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  // sums over a row, the same bits in every thread that has it
+  auto total = [&](auto& t) {
+    g.sum(t);
+    if constexpr (PAIR) {
+      constexpr int M = sizeof(t) / sizeof(float);
+      const uint32_t at = reductions & 1, phase = reductions >> 1 & 1;
+      ++reductions;
+      if (threadIdx.x == 0)
+        cluster_send(&notes.part[at], &notes.bar[at], rank ^ 1, make_float4(t[0], M > 1 ? t[M - 1] : 0.f, 0.f, 0.f));
+      mbar_wait(&notes.bar[at], phase, err, ERR_PEER_FLAG_TIMEOUT, MMF_WAIT_TIMEOUT_NS, false);
+      const float4 other = notes.part[at];
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(&notes.bar[at], sizeof(float4));
+      static_assert(M <= 2, "");
+      t[0] += other.x;
+      if constexpr (M > 1) t[1] += other.y;
+    }
+  };
   const T* pw = static_cast<const T*>(a.post_w);
   const T* pb = static_cast<const T*>(a.post_b);
   const T* nw = static_cast<const T*>(a.pre_w);
@@ -83,7 +127,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   };
   for (int i = 0; i < stages; ++i)
     for (int r = 0; r < ROWS; ++r) clear(i, r);
-  auto col = [&](int k) { return (g.lane + k * tpr) * VEC; };
+  auto col = [&](int k) { return base + (g.lane + k * tpr) * VEC; };
 
   // the worker's rows: chunk after chunk, as many turns for every worker of the block
   const int rounds = (plan.chunks + workers - 1) / workers;
@@ -107,12 +151,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         if (ahead.i + r < ahead.rows) {
-          const int64_t off = static_cast<int64_t>(ahead.first + ahead.i + r) * cols + g.lane * VEC;
+          const int64_t off = static_cast<int64_t>(ahead.first + ahead.i + r) * cols + col(0);
           R* to = place(put, r);
           auto fetch = [&](int i, const void* from) {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
-              if (col(k) < cols)
+              if (col(k) < end)
                 copy_ahead<T, VEC>(to + (i * NV + k) * threads, static_cast<const T*>(from) + off + k * tpr * VEC);
           };
           if (nw) {
@@ -136,7 +180,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
     v.fill(1.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (col(k) >= cols)
+      if (col(k) >= end)
         v.template put<T, VEC>(k, R{});
       else if (p)
         v.template put<T, VEC>(k, ld_raw<T, VEC>(static_cast<const T*>(p) + col(k)));
@@ -145,7 +189,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   auto flush = [&](const V& v, float* to) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (col(k) < cols) {
+      if (col(k) < end) {
         constexpr int P = VEC < 4 ? VEC : 4;
 #pragma unroll
         for (int e = 0; e < VEC; e += P) {
@@ -175,7 +219,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
     for (int i = 0; i < H; ++i) to.p[i] = fmul2(both(a.branch_scale), fmul2(gate.p[i], to.p[i]));
   };
   [[maybe_unused]] V kept_pre, kept_scale, kept_shift;
-  if constexpr (KEEP) column(nw, kept_pre);
+  column(nw, kept_pre);
   const float inv = 1.f / cols;
   const int rows_per_gate = static_cast<int>(a.rows_per_gate);
   auto load_stats = [&](const Cursor& c, Stat (&y)[ROWS], Stat (&h)[ROWS]) {
@@ -202,47 +246,25 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
       const int64_t off = static_cast<int64_t>(now.first + now.i + r) * cols;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (now.i + r < now.rows && col(k) < cols)
+        if (now.i + r < now.rows && col(k) < end)
           st_raw<T, VEC>(static_cast<T*>(to) + off + col(k), v.template get<T, VEC>(k));
     };
-    auto load_gate = [&](int r, V& gate) {
-      if (token_gate)
-        input(r, IN_GATE, gate);
-      else  // the chunk's
-        column(gated ? static_cast<const T*>(a.gate) + static_cast<int64_t>(now.rows > 0 ? now.first / rows_per_gate : 0) * cols
-                     : nullptr, gate);
-    };
-    if constexpr (KEEP) {
-      if (now.i == 0 && !token_gate) {
-        V gate;
-        load_gate(0, gate);
-        times(gate, pw, kept_scale);
-        if constexpr (LN) times(gate, pb, kept_shift);
-      }
+    if (now.i == 0) {  // of a chunk; where each row has its own gate that comes in with the row
+      V gate;
+      column(gated && !token_gate
+                 ? static_cast<const T*>(a.gate) + static_cast<int64_t>(now.rows > 0 ? now.first / rows_per_gate : 0) * cols
+                 : nullptr, gate);
+      times(gate, pw, kept_scale);
+      if constexpr (LN) times(gate, pb, kept_shift);
     }
-    auto load_scale = [&](int r, V& v) {
-      if (KEEP && !token_gate) {
-        v = kept_scale;
-      } else {
+    auto with_gate = [&](int r, const V& kept, V& v) {
+      v = kept;
+      if (token_gate) {
         V gate;
-        load_gate(r, gate);
-        times(gate, pw, v);
+        input(r, IN_GATE, gate);
+#pragma unroll
+        for (int i = 0; i < H; ++i) v.p[i] = fmul2(gate.p[i], v.p[i]);
       }
-    };
-    auto load_shift = [&](int r, V& v) {
-      if (KEEP && !token_gate) {
-        v = kept_shift;
-      } else {
-        V gate;
-        load_gate(r, gate);
-        times(gate, pb, v);
-      }
-    };
-    auto load_pre = [&](V& v) {
-      if constexpr (KEEP)
-        v = kept_pre;
-      else
-        column(nw, v);
     };
     // the next rows' statistics are on their way while these are used
     Stat sy[ROWS], sh[ROWS];
@@ -266,11 +288,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
     };
     auto load_h = [&](int r, const V& u, V& h) {  // h^
       V w;
-      load_scale(r, w);
+      with_gate(r, kept_scale, w);
 #pragma unroll
       for (int i = 0; i < H; ++i) h.p[i] = fmul2(u.p[i], w.p[i]);
       if (LN && pb) {
-        load_shift(r, w);
+        with_gate(r, kept_shift, w);
 #pragma unroll
         for (int i = 0; i < H; ++i) h.p[i] = fadd2(h.p[i], w.p[i]);
       }
@@ -292,21 +314,19 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
         load_y(r, u[r]);
         load_h(r, u[r], h[r]);
         input(r, IN_DN, d[r]);
-        V pre;
-        load_pre(pre);
         float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
         for (int i = 0; i < H; ++i) {
           sum_n.p[i] = ffma2(d[r].p[i], h[r].p[i], sum_n.p[i]);
           if constexpr (LN) sum_nb.p[i] = fadd2(d[r].p[i], sum_nb.p[i]);
-          d[r].p[i] = fmul2(d[r].p[i], pre.p[i]);
+          d[r].p[i] = fmul2(d[r].p[i], kept_pre.p[i]);
           if (LN) s1 = fadd2(d[r].p[i], s1);
           s2 = ffma2(d[r].p[i], h[r].p[i], s2);
         }
         t[r * SUMS] = s2.x + s2.y;
         if constexpr (LN) t[r * SUMS + 1] = s1.x + s1.y;
       }
-      g.sum(t);
+      total(t);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         V dh;
@@ -337,19 +357,17 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
       }
       if (token_gate) {
         // each row's own gate: its gradient goes out with the row, A and B take it in
-        V gate, w, x;
+        V gate, x;
         input(r, IN_GATE, gate);
         if (a.dgate) {
-          column(pw, w);
 #pragma unroll
-          for (int i = 0; i < H; ++i) x.p[i] = fmul2(w.p[i], u[r].p[i]);
+          for (int i = 0; i < H; ++i) x.p[i] = fmul2(kept_scale.p[i], u[r].p[i]);
           if (LN && pb) {
-            column(pb, w);
 #pragma unroll
-            for (int i = 0; i < H; ++i) x.p[i] = fadd2(x.p[i], w.p[i]);
+            for (int i = 0; i < H; ++i) x.p[i] = fadd2(x.p[i], kept_shift.p[i]);
           }
 #pragma unroll
-          for (int i = 0; i < H; ++i) x.p[i] = fmul2(both(a.branch_scale), fmul2(x.p[i], d[r].p[i]));
+          for (int i = 0; i < H; ++i) x.p[i] = fmul2(x.p[i], d[r].p[i]);
           store(r, a.dgate, x);
         }
 #pragma unroll
@@ -366,7 +384,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
         }
       }
       V scale;
-      load_scale(r, scale);
+      with_gate(r, kept_scale, scale);
       float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
       for (int i = 0; i < H; ++i) {
@@ -377,7 +395,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
       t[r * SUMS] = s2.x + s2.y;
       if constexpr (LN) t[r * SUMS + 1] = s1.x + s1.y;
     }
-    if (pw) g.sum(t);
+    if (pw) total(t);
     if (a.dy) {
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
@@ -483,22 +501,22 @@ constexpr int kSharedMost = 224 << 10;
 
 // The launch of a width: what it needs of the device, and how rows are dealt out.
 struct Backward {
-  static constexpr int kValues = 8;  // a thread, while the row needs no more than kMaxThreads
+  static constexpr int kValues = 8;  // a thread
   const BlockNormBwdArgs& a;
   cudaStream_t stream;
   int64_t* need;  // non-null: only count the scratch values
 
-  template <typename T, int VEC, int NV, bool LN>
+  template <typename T, int VEC, int NV, bool LN, bool PAIR = false>
   void run(int tpr) const {
-    auto kernel = block_norm_bwd_kernel<T, VEC, NV, LN>;
-    const int groups = tpr < 128 ? 128 / tpr : 1, block = groups * tpr;  // narrow rows: several to a block
+    auto kernel = block_norm_bwd_kernel<T, VEC, NV, LN, PAIR>;
+    const int groups = !PAIR && tpr < 128 ? 128 / tpr : 1, block = groups * tpr;  // narrow rows: several to a block
     // two rows copied ahead, one or none where they are too wide for that
     const int inputs = a.gate && a.rows_per_gate == 1 ? INPUTS : INPUTS - 1;
-    const int stage = kRows<NV * VEC, LN> * inputs * NV * VEC * static_cast<int>(sizeof(T)) * block;
+    const int stage = kRows<LN> * inputs * NV * VEC * static_cast<int>(sizeof(T)) * block;
     const int stages = std::max(1, std::min(3, kSharedMost / stage));
     const int smem = stages * stage;
     const int per_sm = resident_blocks(reinterpret_cast<const void*>(kernel), block, smem);
-    const int most = 148 * per_sm * groups;  // workers on the device at once
+    const int most = 148 * per_sm * groups / (PAIR ? 2 : 1);  // workers on the device at once
     Plan p;
     const bool shared_gate = a.gate && a.rows_per_gate > 1, gate_sum = shared_gate && a.dgate;
     p.groups = static_cast<int>(shared_gate ? a.rows / a.rows_per_gate : 1);
@@ -528,7 +546,20 @@ struct Backward {
       *need = used;
       return;
     }
-    kernel<<<static_cast<unsigned>(workers / groups), block, smem, stream>>>(a, p, parts, tpr, inputs, stages);
+    int device = 0;
+    cudaGetDevice(&device);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * workers : workers / groups));
+    cfg.blockDim = dim3(static_cast<unsigned>(block));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kernel, a, p, parts, tpr, inputs, stages, device_error_word(device));
     check("block_norm_bwd");
 
     SumJobs jobs{};

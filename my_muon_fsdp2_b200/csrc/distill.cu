@@ -442,16 +442,6 @@ __device__ __forceinline__ Part slice_part(const uint4* slice, int n, bool has_e
   return warp_join<MODE, 32>(part, c_a);
 }
 
-// 16 bytes to the same place in another block's shared memory, counted on that block's barrier.
-__device__ __forceinline__ void send(const void* to, uint64_t* bar, int block, float4 v) {
-  uint32_t remote, remote_bar;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(to)), "r"(block));
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote_bar) : "r"(smem_u32(bar)), "r"(block));
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(remote),
-               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(remote_bar)
-               : "memory");
-}
-
 // One row a cluster.  Shared memory: the block's slice of the row, then the row's slots.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kThreads, 6) distill_rows_kernel(const DistillArgs a, const Scales sc, int each, int* err) {
@@ -506,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 6) distill_rows_kernel(const Distill
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (tid < 32) {
     const Part p = warp_join<MODE, kWarps>(warp_part[lane % kWarps], c_a);
-    if (lane < (whole ? blocks : 1)) send(&block_part[rank], &received, lane, make_float4(p.m, p.s, p.h, 0.f));
+    if (lane < (whole ? blocks : 1)) cluster_send(&block_part[rank], &received, lane, make_float4(p.m, p.s, p.h, 0.f));
   }
   if (!whole && rank != 0) return;
   const int owned = sc.soft > 0.f ? fill_slots(a, sc.c_tau, t, notes, share) : -1;

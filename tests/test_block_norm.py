@@ -349,3 +349,14 @@ def test_gpu_refusals():
                 lambda: f(x.double(), x.double()), lambda: f(x, x.cpu()), lambda: f(x, x, w.cpu())):
         with pytest.raises(TypeError):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("layer", [False, True], ids=["rms", "layer"])
+@pytest.mark.parametrize("D", [4098, 5000, 8192])
+def test_gpu_wide_rows_in_many_turns(D, layer, dtype):
+    """Rows shared by two blocks, more of them than go over the device at once, and each gate."""
+    for n, (gate, lead) in enumerate([("channel", (2, 301)), ("token", (601,)), ("sequence", (3, 211)), ("sequence", (300, 2)), (None, (500,))]):
+        args = _inputs(lead, D, dtype, layer, gate, True, True, "cuda", seed=n)
+        _compare(args, layer)
