@@ -162,18 +162,25 @@ __device__ __forceinline__ Stat row_stat(RowGroup& g, const Values<N>& v, int co
 constexpr int kMaxCols = 8192;
 constexpr int kMaxThreads = 512;
 
-// The columns of the first of two blocks that share a row.
-__host__ __device__ __forceinline__ int first_half(int cols, int vec) { return (cols + 2 * vec - 1) / (2 * vec) * vec; }
+// The columns of each of the blocks that share a row (the last has what is left).
+__host__ __device__ __forceinline__ int share_of(int cols, int blocks, int vec) {
+  return (cols + blocks * vec - 1) / (blocks * vec) * vec;
+}
 
 // Calls go.run<T, VEC, NV, LN>(threads a row) for the widest access that divides the rows' width and
 // their starts (16 bytes, else 4, else one value), with Go::kValues values a thread (VEC at least); where
-// kMaxThreads threads are too few for that, go.run<T, VEC, NV, LN, true>(threads of half a row).
+// kMaxThreads threads are too few for that, go.run<T, VEC, NV, LN, B>(threads of a block's share) with B
+// blocks a row, 2 or 4.
 template <typename T, bool LN, int VEC, typename Go>
 void dispatch_row_width(const Go& go, int cols) {
   constexpr int NV = Go::kValues > VEC ? Go::kValues / VEC : 1;
   auto threads = [&](int n) { return ((n + NV * VEC - 1) / (NV * VEC) + 31) / 32 * 32; };
-  if (cols <= kMaxThreads * NV * VEC) return go.template run<T, VEC, NV, LN>(threads(cols));
-  if constexpr (kMaxThreads * NV * VEC < kMaxCols) go.template run<T, VEC, NV, LN, true>(threads(first_half(cols, VEC)));
+  constexpr int most = kMaxThreads * NV * VEC;
+  if (cols <= most) return go.template run<T, VEC, NV, LN>(threads(cols));
+  if constexpr (most < kMaxCols) {
+    if (Go::four_blocks(cols)) return go.template run<T, VEC, NV, LN, 4>(threads(share_of(cols, 4, VEC)));
+    go.template run<T, VEC, NV, LN, 2>(threads(share_of(cols, 2, VEC)));
+  }
 }
 template <typename T, bool LN, typename Go>
 void dispatch_row_vec(const Go& go, const void* const* rows, int n, int cols) {

@@ -17,14 +17,15 @@
 // threads that shares a row) walks over a run of rows, whose data are copied ahead into shared memory,
 // each thread its own vectors, so that others are on their way while it is at one or two rows' two
 // reductions.  Sums over rows stay in registers, 8 columns a thread, and leave once, as one partial row a
-// worker (one a run for the gate).  Rows of more than 8 x 512 columns are shared by two blocks of a
-// cluster, which exchange the sums of their halves: 8192 x 8192 bf16 240 us (gate for each token 287),
-// where one block with 16 columns a thread had no registers left for the weights, 330 (303).  A second
-// kernel adds the partials in a fixed order, so that equal calls give equal bits.  8192 x 4096 bf16 with
-// both norms and a gate: 90 us, and 5.5 for the sums (403 MB, 69 % of the copy rate); the arithmetic,
-// through packed fp32 instructions, takes about as long as the copies.  With one row a turn 5 us more;
-// unpacked arithmetic, sums in shared memory and no copies ahead 152; 16 columns a thread and two blocks
-// an SM, weights loaded again for each row, 140.
+// worker (one a run for the gate).  Rows of more than 8 x 512 columns are shared by the blocks of a
+// cluster, which exchange the sums of their shares: 8192 x 8192 bf16 233 us (gate for each token 281),
+// where one block with 16 columns a thread had no registers left for the weights, 330 (303).  Narrower rows
+// are not: at 4096 columns two blocks took 126 us, the exchange being slower than one block's barrier.  A
+// second kernel adds the partials in a fixed order, so that equal calls give equal bits.  8192 x 4096 bf16
+// with both norms and a gate: 92 us, and 5.5 for the sums (403 MB, 67 % of the copy rate); the
+// arithmetic, through packed fp32 instructions, takes about as long as the copies.  With one row a turn 5 us
+// more; unpacked arithmetic, sums in shared memory and no copies ahead 152; 16 columns a thread and two
+// blocks an SM, weights loaded again for each row, 140.
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -55,16 +56,17 @@ enum { IN_DN, IN_DH, IN_X, IN_Y, IN_GATE, INPUTS };
 template <bool LN>
 constexpr int kRows = LN ? 1 : 2;
 
-// What two blocks that share a row tell one another: the sums of their halves, an asynchronous store that
-// counts its bytes on the receiver's barrier.  Two places in turn: a block that is one reduction ahead
-// has this one's part of that reduction, which this block sends when all its threads have read the last.
-struct PairNotes {
-  float4 part[2];
+// What blocks that share a row tell one another: the sums of their shares, asynchronous stores that
+// count their bytes on the receiver's barrier.  Two places in turn: a block that is one reduction ahead
+// has the others' parts of that one, which they send when all their threads have read the last.
+template <int BLOCKS>
+struct Shares {
+  float2 part[2][BLOCKS];
   uint64_t bar[2];
 };
 
-// PAIR: a cluster of two blocks shares each row, half the columns each.
-template <typename T, int VEC, int NV, bool LN, bool PAIR>
+// BLOCKS: of a cluster that shares each row, as many columns each (1: a row has one block, or less).
+template <typename T, int VEC, int NV, bool LN, int BLOCKS>
 __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const BlockNormBwdArgs a, const Plan plan,
                                                                         const BwdParts parts, int tpr, int inputs,
                                                                         int stages, int* err) {
@@ -77,20 +79,20 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   RowGroup g(tpr, red);
   const int cols = a.cols, threads = static_cast<int>(blockDim.x);
   const int groups = threads / tpr;
-  const int rank = PAIR ? static_cast<int>(blockIdx.x) & 1 : 0;
-  const int worker = PAIR ? static_cast<int>(blockIdx.x) >> 1 : static_cast<int>(blockIdx.x) * groups + g.row;
-  const int workers = PAIR ? static_cast<int>(gridDim.x) >> 1 : static_cast<int>(gridDim.x) * groups;
+  const int rank = BLOCKS > 1 ? static_cast<int>(blockIdx.y) : 0;
+  const int worker = static_cast<int>(blockIdx.x) * groups + g.row, workers = static_cast<int>(gridDim.x) * groups;
   // the block's columns
-  const int base = rank ? first_half(cols, VEC) : 0, end = PAIR && !rank ? first_half(cols, VEC) : cols;
-  __shared__ PairNotes notes;
+  const int share = BLOCKS > 1 ? share_of(cols, BLOCKS, VEC) : cols, base = rank * share, end = min(base + share, cols);
+  __shared__ Shares<BLOCKS> notes;
+  [[maybe_unused]] constexpr uint32_t kBytes = (BLOCKS - 1) * sizeof(float2);  // of the others' parts
   [[maybe_unused]] uint32_t reductions = 0;
-  if constexpr (PAIR) {
+  if constexpr (BLOCKS > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&notes.bar[0], 1);
       mbar_init(&notes.bar[1], 1);
       fence_mbar_init();
-      mbar_arrive_expect_tx(&notes.bar[0], sizeof(float4));
-      mbar_arrive_expect_tx(&notes.bar[1], sizeof(float4));
+      mbar_arrive_expect_tx(&notes.bar[0], kBytes);
+      mbar_arrive_expect_tx(&notes.bar[1], kBytes);
     }
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -99,18 +101,21 @@ __global__ void __launch_bounds__(kMaxThreads, 1) block_norm_bwd_kernel(const Bl
   // sums over a row, the same bits in every thread that has it
   auto total = [&](auto& t) {
     g.sum(t);
-    if constexpr (PAIR) {
+    if constexpr (BLOCKS > 1) {
       constexpr int M = sizeof(t) / sizeof(float);
       const uint32_t at = reductions & 1, phase = reductions >> 1 & 1;
       ++reductions;
-      if (threadIdx.x == 0)
-        cluster_send(&notes.part[at], &notes.bar[at], rank ^ 1, make_float4(t[0], M > 1 ? t[M - 1] : 0.f, 0.f, 0.f));
-      mbar_wait(&notes.bar[at], phase, err, ERR_PEER_FLAG_TIMEOUT, MMF_WAIT_TIMEOUT_NS, false);
-      const float4 other = notes.part[at];
-      if (threadIdx.x == 0) mbar_arrive_expect_tx(&notes.bar[at], sizeof(float4));
       static_assert(M <= 2, "");
-      t[0] += other.x;
-      if constexpr (M > 1) t[1] += other.y;
+      const float2 mine = make_float2(t[0], t[M - 1]);
+      if (threadIdx.x < BLOCKS && static_cast<int>(threadIdx.x) != rank)
+        cluster_send(&notes.part[at][rank], &notes.bar[at], static_cast<int>(threadIdx.x), mine);
+      mbar_wait(&notes.bar[at], phase, err, ERR_PEER_FLAG_TIMEOUT, MMF_WAIT_TIMEOUT_NS, false);
+      float2 sum = make_float2(0.f, 0.f);  // in the order of the blocks, the same in each of them
+#pragma unroll
+      for (int i = 0; i < BLOCKS; ++i) sum = fadd2(sum, i == rank ? mine : notes.part[at][i]);
+      t[0] = sum.x;
+      if constexpr (M > 1) t[1] = sum.y;
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(&notes.bar[at], kBytes);
     }
   };
   const T* pw = static_cast<const T*>(a.post_w);
@@ -502,21 +507,27 @@ constexpr int kSharedMost = 224 << 10;
 // The launch of a width: what it needs of the device, and how rows are dealt out.
 struct Backward {
   static constexpr int kValues = 8;  // a thread
+  // Whether four blocks take a row that is too wide for one: four with up to 5 warps each, of which an SM holds three,
+  // else two.  8192 x 5120 bf16 157 us with four and 198 with two (layer norms 232 and 316), 8192 x 6144, where an
+  // SM holds two of four, 224 and 202.
+  static bool four_blocks(int cols) { return cols <= 4 * 160 * kValues; }
   const BlockNormBwdArgs& a;
   cudaStream_t stream;
   int64_t* need;  // non-null: only count the scratch values
 
-  template <typename T, int VEC, int NV, bool LN, bool PAIR = false>
+  template <typename T, int VEC, int NV, bool LN, int BLOCKS = 1>
   void run(int tpr) const {
-    auto kernel = block_norm_bwd_kernel<T, VEC, NV, LN, PAIR>;
-    const int groups = !PAIR && tpr < 128 ? 128 / tpr : 1, block = groups * tpr;  // narrow rows: several to a block
-    // two rows copied ahead, one or none where they are too wide for that
+    auto kernel = block_norm_bwd_kernel<T, VEC, NV, LN, BLOCKS>;
+    const int groups = BLOCKS == 1 && tpr < 128 ? 128 / tpr : 1, block = groups * tpr;  // narrow rows: several to a block
+    // two turns' rows copied ahead, one or none where they are too wide for that; small blocks leave room for
+    // a second one on the SM (8192 x 2048 bf16 with a gate for each token: 56 us, 80 with one and three stages)
     const int inputs = a.gate && a.rows_per_gate == 1 ? INPUTS : INPUTS - 1;
     const int stage = kRows<LN> * inputs * NV * VEC * static_cast<int>(sizeof(T)) * block;
-    const int stages = std::max(1, std::min(3, kSharedMost / stage));
+    const int stages = std::max(1, std::min(3, kSharedMost / (block <= 256 ? 2 : 1) / stage));
     const int smem = stages * stage;
-    const int per_sm = resident_blocks(reinterpret_cast<const void*>(kernel), block, smem);
-    const int most = 148 * per_sm * groups / (PAIR ? 2 : 1);  // workers on the device at once
+    // workers on the device at once
+    const void* k = reinterpret_cast<const void*>(kernel);
+    const int most = BLOCKS > 1 ? resident_clusters(k, block, smem, BLOCKS) : 148 * resident_blocks(k, block, smem) * groups;
     Plan p;
     const bool shared_gate = a.gate && a.rows_per_gate > 1, gate_sum = shared_gate && a.dgate;
     p.groups = static_cast<int>(shared_gate ? a.rows / a.rows_per_gate : 1);
@@ -549,16 +560,16 @@ struct Backward {
     int device = 0;
     cudaGetDevice(&device);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * workers : workers / groups));
+    cfg.gridDim = dim3(static_cast<unsigned>(workers / groups), BLOCKS);
     cfg.blockDim = dim3(static_cast<unsigned>(block));
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    attr.val.clusterDim.x = attr.val.clusterDim.z = 1;
+    attr.val.clusterDim.y = BLOCKS;
     cfg.attrs = &attr;
-    cfg.numAttrs = PAIR ? 1 : 0;
+    cfg.numAttrs = BLOCKS > 1 ? 1 : 0;
     cudaLaunchKernelEx(&cfg, kernel, a, p, parts, tpr, inputs, stages, device_error_word(device));
     check("block_norm_bwd");
 

@@ -13,6 +13,7 @@ namespace {
 std::mutex lock;
 std::map<std::pair<const void*, int>, int> allowed;                     // (kernel, device): bytes
 std::map<std::tuple<const void*, int, int, int>, int> resident;         // (kernel, device, block, smem): blocks
+std::map<std::tuple<const void*, int, int, int, int>, int> clusters;    // (the same and blocks a cluster): clusters
 
 void check(cudaError_t e) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("mmf: preparing a kernel: ") + cudaGetErrorString(e));
@@ -53,6 +54,29 @@ int resident_blocks(const void* kernel, int block, int smem) {
   check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, block, static_cast<size_t>(smem)));
   if (blocks < 1) throw std::runtime_error("mmf: preparing a kernel: no block of it fits an SM");
   return resident[key] = blocks;
+}
+
+int resident_clusters(const void* kernel, int block, int smem, int blocks) {
+  const int device = current_device();
+  std::lock_guard<std::mutex> hold(lock);
+  const auto key = std::make_tuple(kernel, device, block, smem, blocks);
+  const auto it = clusters.find(key);
+  if (it != clusters.end()) return it->second;
+  allow(kernel, device, smem, false);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1024, static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(block));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = attr.val.clusterDim.z = 1;
+  attr.val.clusterDim.y = static_cast<unsigned>(blocks);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  check(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+  if (n < 1) throw std::runtime_error("mmf: preparing a kernel: no cluster of it fits the device");
+  return clusters[key] = n;
 }
 
 }  // namespace mmf

@@ -14,4 +14,8 @@ void allow_shared(const void* kernel, int smem, bool carveout = false);
 // or it throws); allow_shared included.
 int resident_blocks(const void* kernel, int block, int smem);
 
+// Clusters of `blocks` such blocks (along y) that the current device holds at once: where a cluster's blocks
+// have to be near one another that is less than the blocks alone would make.
+int resident_clusters(const void* kernel, int block, int smem, int blocks);
+
 }  // namespace mmf

@@ -84,6 +84,15 @@ __device__ __forceinline__ void cluster_send(const void* to, uint64_t* bar, int 
                "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(remote_bar)
                : "memory");
 }
+// The same with 8 bytes.
+__device__ __forceinline__ void cluster_send(const void* to, uint64_t* bar, int block, float2 v) {
+  uint32_t remote, remote_bar;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(to)), "r"(block));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote_bar) : "r"(smem_u32(bar)), "r"(block));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(remote),
+               "f"(v.x), "f"(v.y), "r"(remote_bar)
+               : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
