@@ -360,3 +360,30 @@ def test_gpu_wide_rows_in_many_turns(D, layer, dtype):
     for n, (gate, lead) in enumerate([("channel", (2, 301)), ("token", (601,)), ("sequence", (3, 211)), ("sequence", (300, 2)), (None, (500,))]):
         args = _inputs(lead, D, dtype, layer, gate, True, True, "cuda", seed=n)
         _compare(args, layer)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [5120, 8192])
+def test_gpu_wide_rows_same_bits_streams_and_graph(D):
+    """Rows over several blocks: two calls at once, a captured one and its replay give the same bits."""
+    t = _inputs((2, 331), D, torch.bfloat16, False, "token", True, True, "cuda")
+    a = _run(t, False, 1e-5, 1.0, 1.0)
+    streams, runs = [torch.cuda.Stream() for _ in range(2)], []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            runs.append(_run(t, False, 1e-5, 1.0, 1.0))
+    for st in streams:
+        torch.cuda.current_stream().wait_stream(st)
+    assert all(torch.equal(a[k], r[k]) for r in runs for k in a)
+    del a, runs
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = _run(t, False, 1e-5, 1.0, 1.0)
+    t["y"].mul_(0.5)
+    g.replay()
+    torch.cuda.synchronize()
+    got = {k: v.clone() for k, v in out.items()}
+    del out, g
+    want = _run(t, False, 1e-5, 1.0, 1.0)
+    assert all(torch.equal(got[k], want[k]) for k in want)
