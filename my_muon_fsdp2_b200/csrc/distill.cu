@@ -21,9 +21,12 @@
 // widening them, and at tau = 2 the softmax at 1 comes from the one at tau as its square (one
 // exponential a value instead of two: 236 instead of 320 us at 2048 rows).
 //
-// Every exponential is 2^(c z - R), one fused multiply-add before it.  The reference R is the rounded
-// product c max(z) of a thread, later of the row, and is itself what sums are kept against: its
-// rounding cancels.  Sums are scaled by 2^(R - R') as they are joined, so nothing overflows.
+// Every exponential is 2^(c (z - m)), m the largest logit of a thread, later of the row.  The difference comes
+// first: it is exactly 0 at the maximum, however far that is from 0 (a row whose words are all at the type's
+// lowest value is uniform).  2^(c z - R) with R = c m rounded beforehand is one packed instruction less (1.5 %
+// of the case above), but has R's rounding in its exponent: 440 at z = -1e10, and infinities behind it; with
+// both forms, chosen by |c m|, the case took 1.1 % more all the same.  Sums are scaled by 2^(c (m - m')) as they
+// are joined, so nothing overflows.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -106,18 +109,12 @@ __device__ __forceinline__ int look_at(const DistillArgs& a, int64_t y, int* err
 }
 
 // The largest of some logits, and the sums of their exponentials at the temperature of c_a (s) and, in
-// the modes that have them, at 1 (h), against the references of that maximum.
+// the modes that have them, at 1 (h), relative to that maximum.
 struct Part {
   float m, s, h;
-};
-template <int MODE>
-struct Reference {
-  float a, b;
-  __device__ __forceinline__ Reference(float m, float c_a) {
-    if (m == -INFINITY) m = 0.f;  // nothing but -inf (or NaN, which the sums carry): every term is 0
-    a = __fmul_rn(m, c_a);
-    b = MODE == TWO ? __fmul_rn(m, kLog2e) : 2.f * a;
-  }
+  // What is taken off a logit: the maximum, or 0 where there is nothing but -inf (or NaN, which the sums
+  // carry), so that every term is 0.
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
 };
 // Over groups of `W` lanes, the same bits in each of them.
 template <int MODE, int W>
@@ -125,10 +122,10 @@ __device__ __forceinline__ Part warp_join(Part p, float c_a) {
   float m = p.m;
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const Reference<MODE> from(p.m, c_a), to(m, c_a);
-  // without a finite logit of its own a part is 0 (or NaN) against any reference
-  p.s *= p.m == -INFINITY ? 1.f : ex2(from.a - to.a);
-  if (MODE != ONE) p.h *= p.m == -INFINITY ? 1.f : ex2(from.b - to.b);
+  // without a finite logit of its own a part is 0 (or NaN) against any maximum
+  const float down = p.m == -INFINITY ? 0.f : p.m - m;
+  p.s *= ex2(down * c_a);
+  if (MODE != ONE) p.h *= ex2(down * kLog2e);
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1) {
     p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
@@ -344,22 +341,20 @@ struct Coefficients {
 // reciprocals are in the factors.
 template <int MODE>
 struct Dense {
-  float2 c, r_a, r_b, log2e, f_a, f_b;
+  float2 c, off, log2e, f_a, f_b;
   __device__ __forceinline__ Dense(const Coefficients& k, float c_a, const Part& p) {
-    const Reference<MODE> r(p.m, c_a);
     c = make_float2(c_a, c_a);
-    r_a = make_float2(-r.a, -r.a);
-    r_b = make_float2(-r.b, -r.b);
+    off = make_float2(-p.base(), -p.base());
     log2e = make_float2(kLog2e, kLog2e);
     const float a = __fdividef(k.k_a, p.s), b = MODE == ONE ? 0.f : __fdividef(k.k_b, p.h);
     f_a = make_float2(a, a);
     f_b = make_float2(b, b);
   }
   __device__ __forceinline__ float2 operator()(float2 z) const {
-    const float2 e = exp2_2(ffma2(z, c, r_a));
+    const float2 d = fadd2(z, off), e = exp2_2(fmul2(d, c));
     if (MODE == ONE) return fmul2(e, f_a);
     if (MODE == SQUARE) return fmul2(e, ffma2(e, f_b, f_a));
-    return ffma2(exp2_2(ffma2(z, log2e, r_b)), f_b, fmul2(e, f_a));
+    return ffma2(exp2_2(fmul2(d, log2e)), f_b, fmul2(e, f_a));
   }
   __device__ __forceinline__ float one(float z) const { return (*this)(make_float2(z, z)).x; }
 };
@@ -419,15 +414,14 @@ __device__ __forceinline__ Part slice_part(const uint4* slice, int n, bool has_e
   for (int i = threadIdx.x; i < n; i += kThreads) most.put(slice[i]);
   Part part{most.get(), 0.f, 0.f};
   if (has_edge) part.m = fmaxf(part.m, edge);
-  const Reference<MODE> r(part.m, c_a);
-  const float2 r_a = make_float2(-r.a, -r.a), r_b = make_float2(-r.b, -r.b), c = make_float2(c_a, c_a);
+  const float2 off = make_float2(-part.base(), -part.base()), c = make_float2(c_a, c_a);
   const float2 log2e = make_float2(kLog2e, kLog2e);
   float2 s = make_float2(0.f, 0.f), h = s;
   auto term = [&](float2 z) {
-    const float2 e = exp2_2(ffma2(z, c, r_a));
+    const float2 d = fadd2(z, off), e = exp2_2(fmul2(d, c));
     s = fadd2(s, e);
     if (MODE == SQUARE) h = ffma2(e, e, h);
-    if (MODE == TWO) h = fadd2(h, exp2_2(ffma2(z, log2e, r_b)));
+    if (MODE == TWO) h = fadd2(h, exp2_2(fmul2(d, log2e)));
   };
   if (has_edge) term(make_float2(edge, -INFINITY));
 #pragma unroll 4
@@ -511,14 +505,13 @@ __global__ void __launch_bounds__(kThreads, 6) distill_rows_kernel(const Distill
   auto put_loss = [&]() {
     const bool many = a.top > kWarpSlots;  // one warp has few; more are shared by all, which costs a barrier
     if (rank != 0 || (!many && tid >= 32)) return;
-    const Reference<MODE> r(p.m, c_a);
-    const float l_a = log2f(p.s);
+    const float base = p.base(), l_a = log2f(p.s);
     float kd = 0.f;  // sum p_j (log2 p_j - log2 q_tau(id_j))
     if (soft) {
       const float inv = notes.inverse();
       for (int j = tid; j < a.top; j += many ? kThreads : 32) {
         const float p_j = t.p[j] * inv;
-        if (p_j > 0.f) kd = fmaf(p_j, log2f(p_j) - (fmaf(t.z[j], c_a, -r.a) - l_a), kd);
+        if (p_j > 0.f) kd = fmaf(p_j, log2f(p_j) - fmaf(t.z[j] - base, c_a, -l_a), kd);
       }
       kd = warp_sum(kd);
       if (many) {
@@ -528,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 6) distill_rows_kernel(const Distill
       }
     }
     if (tid == 0) {
-      const float ce = kLn2 * (MODE == ONE ? l_a - fmaf(target_z, c_a, -r.a) : log2f(p.h) - fmaf(target_z, kLog2e, -r.b));
+      const float ce = kLn2 * (MODE == ONE ? l_a - (target_z - base) * c_a : log2f(p.h) - (target_z - base) * kLog2e);
       // sub_p = alpha tau / count; the loss has another tau
       a.loss[row] = (soft ? k.sub_p * a.tau * kLn2 * kd : 0.f) + (hard ? k.sub_y * ce : 0.f);
       if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(p.m, p.s, p.h, soft ? 1.f : 0.f);

@@ -423,3 +423,50 @@ def test_gpu_many_slots_of_few_words(N, V, K, dtype):
             runs.append((loss.detach(), *torch.autograd.grad(loss.sum(), z)))
         z = z.detach()
         assert all(torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1]) for r in runs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("tau", [1.0, 2.0, 1.7])
+@pytest.mark.parametrize("value", [-1e10, 1e10, -math.inf, math.inf], ids=["-1e10", "1e10", "lowest", "highest"])
+def test_gpu_rows_far_from_zero(value, tau, dtype):
+    """Rows whose logits are all the same large value, the type's lowest (a mask over the whole row) or highest
+    one among them, are uniform; rows beside them and the mean keep their values.  And rows of large logits
+    that differ."""
+    f = torch.finfo(dtype)
+    value = max(f.min, min(f.max, value))
+    for N, V in ((4, 301), (9, 50257)):
+        z, ids, a, y = _inputs(N, V, 5, torch.float32, "cuda")
+        z[torch.isinf(z)] = 0.0
+        z = z.to(dtype)
+        z[0::2] = value
+        for reduction in ("none", "mean"):
+            _check(z, ids, a, y, tau, 0.5, reduction)
+            _check(z, ids, a, None, tau, 1.0, reduction)
+        if abs(value) == 1e10:
+            z[0::2, ::3] = value * (1 - 2**-6)
+            _check(z, ids, a, y, tau, 0.5, "mean")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tau", [1.0, 2.0, 1.7])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_gpu_rows_around_a_large_value(sign, tau):
+    """Logits a few units apart whose exponents are around 2^12 and 2^20, where the type has few steps left
+    between them."""
+    for N, V, size in ((5, 2003, 2**20), (9, 50257, 2**20), (5, 2003, 2**12)):
+        z, ids, a, y = _inputs(N, V, 5, torch.float32, "cuda")
+        z[torch.isinf(z)] = 0.0
+        z = sign * size * math.log(2.0) * tau + z * torch.linspace(0.25, 4.0, N, device="cuda")[:, None]
+        for reduction in ("none", "mean"):
+            _check(z, ids, a, y, tau, 0.5, reduction)
+            _check(z, ids, a, None, tau, 1.0, reduction)
+
+
+def test_rows_far_from_zero_on_cpu():
+    for value in (-1e10, torch.finfo(torch.float32).min, torch.finfo(torch.float32).max):
+        z, ids, a, y = _inputs(5, 301, 4)
+        z[torch.isinf(z)] = 0.0
+        z[0::2] = value
+        for tau in (1.0, 2.0, 1.7):
+            _check(z, ids, a, y, tau, 0.5, "mean")
