@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 6) distill_rows_kernel(const Distill
       const float inv = notes.inverse();
       for (int j = tid; j < a.top; j += many ? kThreads : 32) {
         const float p_j = t.p[j] * inv;
-        if (p_j > 0.f) kd = fmaf(p_j, log2f(p_j) - fmaf(t.z[j] - base, c_a, -l_a), kd);
+        if (p_j != 0.f) kd = fmaf(p_j, log2f(p_j) - fmaf(t.z[j] - base, c_a, -l_a), kd);  // a teacher's NaN goes through
       }
       kd = warp_sum(kd);
       if (many) {

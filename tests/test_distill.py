@@ -470,3 +470,24 @@ def test_rows_far_from_zero_on_cpu():
         z[0::2] = value
         for tau in (1.0, 2.0, 1.7):
             _check(z, ids, a, y, tau, 0.5, "mean")
+
+
+def _teacher_without_values(device):
+    """A slot whose teacher logit is NaN or +inf makes its token's loss NaN, and no other's."""
+    for bad in (math.nan, math.inf):
+        for K in (4, 300):
+            z, ids, a, y = _inputs(6, 1000, K, torch.float32, device)
+            want = distillation_loss(z, ids, a, y, alpha=0.5, reduction="none")
+            a[0, 1] = bad
+            got = distillation_loss(z, ids, a, y, alpha=0.5, reduction="none")
+            assert got[0].isnan() and torch.equal(got[1:], want[1:])
+            assert distillation_loss(z, ids, a, y, alpha=0.5).isnan()
+
+
+def test_teacher_without_values_on_cpu():
+    _teacher_without_values("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_teacher_without_values():
+    _teacher_without_values("cuda")
