@@ -39,6 +39,13 @@ bool wants_grad(std::initializer_list<const OptTensor*> ts) {
   return false;
 }
 
+// A tangent of forward-mode differentiation does not show in requires_grad: without this it would be lost.
+void refuse_forward_mode(const char* what, std::initializer_list<const OptTensor*> ts) {
+  for (const OptTensor* t : ts)
+    TORCH_CHECK(!t->has_value() || !(*t)->defined() || !(*t)->_fw_grad(/*level=*/0).defined(), "mmf: ", what,
+                " has no forward-mode derivatives");
+}
+
 void refuse_second_order(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "mmf: ", what, " has no second derivatives (create_graph=True)");
 }
@@ -168,6 +175,7 @@ py::object rotary(const Tensor& q, const OptTensor& k, const OptTensor& position
   const bool pair = k.has_value();
   TORCH_CHECK(q.dim() >= 3 && q.size(-1) == head_dim, "mmf: rotary: q must be [..., heads, ", num(head_dim), "]");
   const OptTensor oq(q);
+  refuse_forward_mode("rotary", {&oq, &k});
   const bool grad = wants_grad({&oq, &k});
   if (in_place) {
     TORCH_CHECK(!grad, "mmf: rotary: in place is for tensors outside autograd");
@@ -354,6 +362,7 @@ py::object block_norm(const Tensor& x, const Tensor& y, const OptTensor& pw, con
               "mmf: block_norm: a bias needs its weight and the layer norm");
   const int64_t shared = rows_per_gate(gate, x);
   const OptTensor ox(x), oy(y);
+  refuse_forward_mode("block_norm", {&ox, &oy, &pw, &pb, &gate, &nw, &nb});
   const Tensor xc = x.contiguous(), yc = y.contiguous();
   const OptTensor pwc = dense(pw), pbc = dense(pb), gc = dense(gate), nwc = dense(nw), nbc = dense(nb);
   if (!wants_grad({&ox, &oy, &pw, &pb, &gate, &nw, &nb}))
@@ -564,6 +573,8 @@ Tensor distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, c
                   teacher.sizes() == ids.sizes() && (!targets.has_value() || targets->sizes() == logits.sizes().slice(0, lead)),
               "mmf: distill: the teacher's slots and the targets must have the logits' leading dimensions");
   TORCH_CHECK(!(at::GradMode::is_enabled() && teacher.requires_grad()), "mmf: distill: the teacher takes no gradient");
+  const OptTensor given(logits), of(teacher);
+  refuse_forward_mode("distill", {&given, &of});
   TORCH_CHECK(tau >= 1e-3 && tau <= 1e3 && alpha >= 0 && alpha <= 1 && (alpha == 1 || targets.has_value()),
               "mmf: distill: temperature, alpha or targets out of range");
   const int64_t vocab = logits.size(-1), top = ids.size(-1);

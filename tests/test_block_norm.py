@@ -387,3 +387,32 @@ def test_gpu_wide_rows_same_bits_streams_and_graph(D):
     del out, g
     want = _run(t, False, 1e-5, 1.0, 1.0)
     assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+def _duals(call, shapes, device):
+    import torch.autograd.forward_ad as fw
+
+    for name in shapes:
+        with fw.dual_level():
+            ts = {n: torch.ones(s, device=device) for n, s in shapes.items()}
+            ts[name] = fw.make_dual(ts[name], torch.ones_like(ts[name]))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(ts)
+
+
+SHAPES = {"x": (2, 3, 8), "y": (2, 3, 8), "post_weight": (8,), "post_bias": (8,), "gate": (2, 1, 8), "pre_weight": (8,), "pre_bias": (8,)}
+
+
+def test_forward_mode_is_refused_by_the_entry():
+    """A tangent on any of the tensors; the extension refuses it before it looks at where they are."""
+    from my_muon_fsdp2_b200._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    _duals(lambda t: ext().block_norm(*[t[n] for n in NAMES], True, 1e-5, 1.0, 1.0), SHAPES, "cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_forward_mode_is_refused():
+    _duals(lambda t: gated_residual_norm(**t, norm="layer"), SHAPES, "cuda")

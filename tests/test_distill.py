@@ -491,3 +491,35 @@ def test_teacher_without_values_on_cpu():
 @pytest.mark.gpu
 def test_gpu_teacher_without_values():
     _teacher_without_values("cuda")
+
+
+def _dual_logits(call, device):
+    import torch.autograd.forward_ad as fw
+
+    ids = torch.zeros(4, 2, dtype=torch.long, device=device)
+    for dual in ("logits", "teacher"):
+        with fw.dual_level():
+            z, a = torch.ones(4, 16, device=device), torch.ones(4, 2, device=device)
+            if dual == "logits":
+                z = fw.make_dual(z, torch.ones_like(z))
+            else:
+                a = fw.make_dual(a, torch.ones_like(a))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="forward-mode|forward mode"):
+                    call(z, ids, a)
+
+
+def test_forward_mode_is_refused_by_the_entry():
+    from my_muon_fsdp2_b200._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    _dual_logits(lambda z, ids, a: ext().distill(z, ids, a, None, 1.0, 1.0, -100, True), "cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_forward_mode_is_refused():
+    for reduction in ("mean", "none"):
+        _dual_logits(lambda z, ids, a: distillation_loss(z, ids, a, reduction=reduction), "cuda")
+    w = torch.ones(24, 16, device="cuda", dtype=torch.bfloat16)
+    _dual_logits(lambda x, ids, a: fused_linear_distillation(x.bfloat16(), w, ids, a), "cuda")

@@ -320,3 +320,35 @@ def test_gpu_inplace_is_seen_by_autograd():
         q = torch.randn(1, 2, 3, 8, device="cuda")
         want = apply_rotary(q, None, rot)
         assert apply_rotary(q, None, rot, inplace=True) is q and torch.equal(q, want)
+
+
+def _dual_is_refused(call, *shapes, device="cuda"):
+    """call(tensors) raises when any one of them has a tangent, whether or not gradients are recorded."""
+    import torch.autograd.forward_ad as fw
+
+    for i in range(len(shapes)):
+        with fw.dual_level():
+            ts = [torch.ones(s, device=device) for s in shapes]
+            ts[i] = fw.make_dual(ts[i], torch.ones_like(ts[i]))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*ts)
+
+
+def test_forward_mode_is_refused_by_the_entry():
+    """The extension refuses tensors with a tangent before it looks at where they are."""
+    from my_muon_fsdp2_b200._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    rot = RotaryEmbedding(8)
+    for inplace in (False, True):
+        _dual_is_refused(lambda q, k: ext().rotary(q, k, None, rot._turns, 8, 8, False, 1.0, inplace), (1, 2, 3, 8), (1, 2, 1, 8),
+                         device="cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_forward_mode_is_refused():
+    rot = RotaryEmbedding(8)
+    for inplace in (False, True):
+        _dual_is_refused(lambda q, k: apply_rotary(q, k, rot, inplace=inplace), (1, 2, 3, 8), (1, 2, 1, 8))
