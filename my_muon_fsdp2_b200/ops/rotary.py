@@ -84,7 +84,8 @@ class RotaryEmbedding:
         self.frequencies, self.magnitude = self._frequencies()
         # turns per position as 64-bit fixed-point fractions of a turn (kept in int64 bit patterns)
         turns = [int(math.fmod(f / (2 * math.pi), 1.0) * 2**64) for f in self.frequencies]
-        self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64)
+        with torch.inference_mode(False):
+            self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64)
         self._on: Dict[torch.device, torch.Tensor] = {}
 
     def _frequencies(self) -> Tuple[list, float]:
@@ -123,7 +124,9 @@ class RotaryEmbedding:
         if t is None:
             if device.type == "cuda" and device.index is None:
                 return self._table(torch.device("cuda", torch.cuda.current_device()))
-            t = self._on[device] = self._turns.to(device)
+            # a table first used in inference mode is one that a later training step saves for its backward
+            with torch.inference_mode(False):
+                t = self._on[device] = self._turns.to(device)
         return t
 
     def cos_sin(self, positions: torch.Tensor, dtype=torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:

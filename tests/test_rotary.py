@@ -352,3 +352,35 @@ def test_gpu_forward_mode_is_refused():
     rot = RotaryEmbedding(8)
     for inplace in (False, True):
         _dual_is_refused(lambda q, k: apply_rotary(q, k, rot, inplace=inplace), (1, 2, 3, 8), (1, 2, 1, 8))
+
+
+def test_tables_made_in_inference_mode_are_ordinary_tensors():
+    with torch.inference_mode():
+        rot = RotaryEmbedding(8)
+        table = rot._table(torch.device("cpu"))
+    assert not rot._turns.is_inference() and not table.is_inference()
+
+
+@pytest.mark.gpu
+def test_gpu_evaluation_before_training():
+    """The plan's first use, and its making, in inference mode; then a step with gradients."""
+    from my_muon_fsdp2_b200.models.llama import Llama, LlamaConfig
+
+    made = RotaryEmbedding(8)
+    with torch.inference_mode():
+        inside = RotaryEmbedding(8)
+        for rot in (made, inside):
+            apply_rotary(torch.ones(1, 2, 3, 8, device="cuda"), None, rot)
+    q = _rand((1, 2, 3, 8), torch.float32, "cuda").requires_grad_()
+    for rot in (made, inside):
+        out = apply_rotary(q, None, rot)
+        (g,) = torch.autograd.grad(out, q, torch.ones_like(out))
+        _close(g, *_formula(torch.ones_like(q), torch.arange(2, device="cuda")[None], rot, inverse=True))
+    torch.manual_seed(0)
+    model = Llama(LlamaConfig.tiny(dim=128, n_heads=2, n_kv_heads=1, ffn_dim=256, n_layers=1, rope_scaling=SCALINGS[3]))
+    model = model.to("cuda", torch.bfloat16)
+    tokens = torch.randint(0, 512, (2, 17), device="cuda")
+    with torch.inference_mode():
+        model(tokens)
+    model(tokens[:, :-1], tokens[:, 1:]).backward()
+    assert all(p.grad is not None for p in model.parameters())
