@@ -85,7 +85,7 @@ class RotaryEmbedding:
         # turns per position as 64-bit fixed-point fractions of a turn (kept in int64 bit patterns)
         turns = [int(math.fmod(f / (2 * math.pi), 1.0) * 2**64) for f in self.frequencies]
         with torch.inference_mode(False):
-            self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64)
+            self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64, device="cpu")
         self._on: Dict[torch.device, torch.Tensor] = {}
 
     def _frequencies(self) -> Tuple[list, float]:

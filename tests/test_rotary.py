@@ -384,3 +384,23 @@ def test_gpu_evaluation_before_training():
         model(tokens)
     model(tokens[:, :-1], tokens[:, 1:]).backward()
     assert all(p.grad is not None for p in model.parameters())
+
+
+def test_plan_made_under_another_default_device():
+    """A model is often built under the meta device before it is sharded: the plan's table has its values."""
+    want = RotaryEmbedding(8)
+    with torch.device("meta"):
+        rot = RotaryEmbedding(8)
+    assert torch.equal(rot._turns, want._turns)
+    x = _rand((1, 2, 3, 8), torch.float32)
+    assert torch.equal(apply_rotary(x, None, rot), apply_rotary(x, None, want))
+
+
+@pytest.mark.gpu
+def test_gpu_plan_made_under_another_default_device():
+    x = _rand((1, 2, 3, 8), torch.float32, "cuda")
+    want = apply_rotary(x, None, RotaryEmbedding(8))
+    for device in ("meta", "cuda"):
+        with torch.device(device):
+            rot = RotaryEmbedding(8)
+        assert torch.equal(apply_rotary(x, None, rot), want)
