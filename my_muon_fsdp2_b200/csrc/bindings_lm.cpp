@@ -186,11 +186,14 @@ py::object rotary(const Tensor& q, const OptTensor& k, const OptTensor& position
     };
     TORCH_CHECK(own(q) && (!pair || own(*k)) && (!pair || q.numel() == 0 || q.data_ptr() != k->data_ptr()),
                 "mmf: rotary: in place needs contiguous heads in memory of their own");
-    // a backward pass that kept q or k has to see that they have changed
-    if (!q.is_inference()) q.unsafeGetTensorImpl()->bump_version();
-    if (pair && !k->is_inference()) k->unsafeGetTensorImpl()->bump_version();
   }
-  if (!grad) return pair_or_one(rotary_raw(q, k, positions, turns, rotary_dim, interleaved, magnitude, false, in_place), pair);
+  if (!grad) {
+    const auto out = rotary_raw(q, k, positions, turns, rotary_dim, interleaved, magnitude, false, in_place);
+    // a backward pass that kept q or k has to see that they have changed (a refused call leaves them as they were)
+    if (in_place && !q.is_inference()) q.unsafeGetTensorImpl()->bump_version();
+    if (in_place && pair && !k->is_inference()) k->unsafeGetTensorImpl()->bump_version();
+    return pair_or_one(out, pair);
+  }
   return pair_or_one(RotaryFn::apply(q, k, positions, turns, rotary_dim, interleaved, magnitude), pair);
 }
 

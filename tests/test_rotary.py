@@ -404,3 +404,31 @@ def test_gpu_plan_made_under_another_default_device():
         with torch.device(device):
             rot = RotaryEmbedding(8)
         assert torch.equal(apply_rotary(x, None, rot), want)
+
+
+def test_refused_in_place_call_leaves_versions():
+    """The extension refuses CPU tensors: their version counters stay."""
+    from my_muon_fsdp2_b200._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    rot, q, k = RotaryEmbedding(8), torch.zeros(1, 2, 3, 8), torch.zeros(1, 2, 1, 8)
+    with pytest.raises(RuntimeError):
+        ext().rotary(q, k, None, rot._turns, 8, 8, False, 1.0, True)
+    assert q._version == 0 and k._version == 0
+
+
+@pytest.mark.gpu
+def test_gpu_refused_in_place_call_leaves_versions():
+    rot = RotaryEmbedding(8).to("cuda")
+    q, k = torch.randn(1, 2, 3, 8, device="cuda"), torch.randn(1, 2, 1, 8, device="cuda")
+    w = torch.randn(8, 4, device="cuda", requires_grad=True)
+    out = (q @ w).sum() + (k @ w).sum()
+    for bad, error in ((dict(positions=torch.zeros(2, device="cuda")), TypeError), (dict(positions=torch.zeros(3, dtype=torch.long, device="cuda")), ValueError),
+                       (dict(k=k.bfloat16()), ValueError), (dict(k=k[:, :1]), ValueError)):
+        with pytest.raises(error):
+            apply_rotary(q, bad.get("k", k), rot, bad.get("positions"), inplace=True)
+    assert q._version == 0 and k._version == 0
+    torch.autograd.grad(out, w)
+    apply_rotary(q, k, rot, inplace=True)
+    assert q._version == 1 and k._version == 1
