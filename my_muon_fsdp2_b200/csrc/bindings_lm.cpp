@@ -39,6 +39,14 @@ bool wants_grad(std::initializer_list<const OptTensor*> ts) {
   return false;
 }
 
+// Wrappers (a DTensor outside its module's forward, say) have a device and a shape but no memory: their null
+// pointers would read as a missing weight, or fault.
+void check_memory(const char* what, std::initializer_list<const OptTensor*> ts) {
+  for (const OptTensor* t : ts)
+    TORCH_CHECK(!t->has_value() || !(*t)->defined() || (*t)->numel() == 0 || (*t)->data_ptr() != nullptr, "mmf: ", what,
+                " takes tensors that have memory of their own (of a DTensor, its local tensor)");
+}
+
 // A tangent of forward-mode differentiation does not show in requires_grad: without this it would be lost.
 void refuse_forward_mode(const char* what, std::initializer_list<const OptTensor*> ts) {
   for (const OptTensor* t : ts)
@@ -175,6 +183,7 @@ py::object rotary(const Tensor& q, const OptTensor& k, const OptTensor& position
   const bool pair = k.has_value();
   TORCH_CHECK(q.dim() >= 3 && q.size(-1) == head_dim, "mmf: rotary: q must be [..., heads, ", num(head_dim), "]");
   const OptTensor oq(q);
+  check_memory("rotary", {&oq, &k, &positions});
   refuse_forward_mode("rotary", {&oq, &k});
   const bool grad = wants_grad({&oq, &k});
   if (in_place) {
@@ -358,13 +367,14 @@ OptTensor dense(const OptTensor& t) { return t.has_value() ? OptTensor(t->contig
 py::object block_norm(const Tensor& x, const Tensor& y, const OptTensor& pw, const OptTensor& pb, const OptTensor& gate,
                       const OptTensor& nw, const OptTensor& nb, bool layer, double eps, double residual_scale,
                       double branch_scale) {
+  const OptTensor ox(x), oy(y);
+  check_memory("block_norm", {&ox, &oy, &pw, &pb, &gate, &nw, &nb});
   TORCH_CHECK(x.dim() >= 1 && x.sizes() == y.sizes(), "mmf: block_norm: x must be [..., dim] and y of its shape");
   for (const OptTensor* t : {&pw, &pb, &nw, &nb})
     TORCH_CHECK(!t->has_value() || (*t)->dim() == 1, "mmf: block_norm: weights and biases must be [dim]");
   TORCH_CHECK(!(pb.has_value() && !(layer && pw.has_value())) && !(nb.has_value() && !(layer && nw.has_value())),
               "mmf: block_norm: a bias needs its weight and the layer norm");
   const int64_t shared = rows_per_gate(gate, x);
-  const OptTensor ox(x), oy(y);
   refuse_forward_mode("block_norm", {&ox, &oy, &pw, &pb, &gate, &nw, &nb});
   const Tensor xc = x.contiguous(), yc = y.contiguous();
   const OptTensor pwc = dense(pw), pbc = dense(pb), gc = dense(gate), nwc = dense(nw), nbc = dense(nb);
@@ -571,12 +581,13 @@ class DistillFn : public torch::autograd::Function<DistillFn> {
 // logits [..., vocab], ids and teacher [..., top], targets [...]
 Tensor distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const OptTensor& targets, double tau,
                double alpha, int64_t ignore_index, bool mean) {
+  const OptTensor given(logits), slots(ids), of(teacher);
+  check_memory("distill", {&given, &slots, &of, &targets});
   const int64_t lead = logits.dim() - 1;
   TORCH_CHECK(lead >= 0 && ids.dim() == lead + 1 && ids.sizes().slice(0, lead) == logits.sizes().slice(0, lead) &&
                   teacher.sizes() == ids.sizes() && (!targets.has_value() || targets->sizes() == logits.sizes().slice(0, lead)),
               "mmf: distill: the teacher's slots and the targets must have the logits' leading dimensions");
   TORCH_CHECK(!(at::GradMode::is_enabled() && teacher.requires_grad()), "mmf: distill: the teacher takes no gradient");
-  const OptTensor given(logits), of(teacher);
   refuse_forward_mode("distill", {&given, &of});
   TORCH_CHECK(tau >= 1e-3 && tau <= 1e3 && alpha >= 0 && alpha <= 1 && (alpha == 1 || targets.has_value()),
               "mmf: distill: temperature, alpha or targets out of range");

@@ -195,6 +195,8 @@ def fused_linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_ids
         raise ValueError(f"distillation: chunk must be at least 1, got {chunk}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.dtype != weight.dtype or x.device != weight.device:
         raise ValueError("distillation: x must be [..., dim] and weight [vocab, dim], of one dtype and device")
+    if x.is_cuda and any(t is not None and t.numel() and t.data_ptr() == 0 for t in (x, weight, teacher_ids, teacher_logits, targets)):
+        raise RuntimeError("distillation: the kernels take tensors that have memory of their own (of a DTensor, its local tensor)")
     lead = x.shape[:-1]
     if teacher_ids.shape[:-1] != lead or (targets is not None and targets.shape != lead):
         raise ValueError(f"distillation: teacher_ids {tuple(teacher_ids.shape)} and targets must have x's leading "

@@ -209,3 +209,59 @@ def test_gpu_gpt2_distils_with_its_odd_vocabulary():
         if "c_attn.bias" in n:
             continue  # the key bias has no gradient but for roundings
         assert ((g.double().cpu() - w).norm() / w.norm()).item() < 0.05, n
+
+
+class _Wrapper(torch.Tensor):
+    """A tensor with a device and a shape, and no memory, as a DTensor is."""
+
+    @staticmethod
+    def __new__(cls, *shape, dtype=torch.float32):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device="cuda:0")
+
+    @classmethod
+    def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+        return cls(*args[0].shape, dtype=args[0].dtype)
+
+
+def _wrappers_are_refused(device, rotary, norm, loss, fused):
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, device=device, dtype=dtype)  # noqa: E731
+    bf, ids = torch.bfloat16, torch.zeros(4, 2, dtype=torch.long, device=device)
+    w = _Wrapper
+    for call in (lambda: rotary(w(1, 2, 3, 8), z(1, 2, 1, 8), None), lambda: rotary(z(1, 2, 3, 8), w(1, 2, 1, 8), None),
+                 lambda: rotary(z(1, 2, 3, 8), z(1, 2, 1, 8), w(2, dtype=torch.long)),
+                 lambda: norm(w(4, 8), z(4, 8), z(8), z(8), z(8)), lambda: norm(z(4, 8), w(4, 8), z(8), z(8), z(8)),
+                 lambda: norm(z(4, 8), z(4, 8), w(8), z(8), z(8)), lambda: norm(z(4, 8), z(4, 8), z(8), w(8), z(8)),
+                 lambda: norm(z(4, 8), z(4, 8), z(8), z(8), w(8)), lambda: loss(w(4, 16), ids, z(4, 2)),
+                 lambda: loss(z(4, 16), w(4, 2, dtype=torch.long), z(4, 2)), lambda: loss(z(4, 16), ids, w(4, 2)),
+                 lambda: fused(w(4, 8, dtype=bf), w(16, 8, dtype=bf), ids, z(4, 2))):
+        with pytest.raises(RuntimeError, match="memory of their own"):
+            call()
+
+
+def test_wrappers_without_memory_are_refused_by_the_entries():
+    """Before anything is read or launched; the entries look at this first, wherever the tensors are."""
+    from my_muon_fsdp2_b200._ext import available, ext
+    from my_muon_fsdp2_b200.ops.distill import fused_linear_distillation
+    from my_muon_fsdp2_b200.ops.rotary import RotaryEmbedding
+
+    if not available():
+        pytest.skip("the extension is not built")
+    E, turns = ext(), RotaryEmbedding(8)._turns
+    _wrappers_are_refused("cpu", lambda q, k, pos: E.rotary(q, k, pos, turns, 8, 8, False, 1.0, False),
+                          lambda x, y, pw, gate, nw: E.block_norm(x, y, pw, None, gate, nw, None, False, 1e-5, 1.0, 1.0),
+                          lambda z, ids, a: E.distill(z, ids, a, None, 1.0, 1.0, -100, True), fused_linear_distillation)
+
+
+@pytest.mark.gpu
+def test_gpu_wrappers_without_memory_are_refused():
+    from my_muon_fsdp2_b200.ops.block_norm import gated_residual_norm
+    from my_muon_fsdp2_b200.ops.distill import distillation_loss, fused_linear_distillation
+    from my_muon_fsdp2_b200.ops.rotary import RotaryEmbedding, apply_rotary
+
+    rot = RotaryEmbedding(8).to("cuda")
+    x, w = torch.zeros(4, 8, device="cuda", dtype=torch.bfloat16), _Wrapper(16, 8, dtype=torch.bfloat16)
+    _wrappers_are_refused("cuda", lambda q, k, pos: apply_rotary(q, k, rot, pos),
+                          lambda x, y, pw, gate, nw: gated_residual_norm(x, y, pw, gate=gate, pre_weight=nw), distillation_loss,
+                          fused_linear_distillation)
+    with pytest.raises(RuntimeError, match="memory of their own"):
+        fused_linear_distillation(x, w, torch.zeros(4, 2, dtype=torch.long, device="cuda"), torch.zeros(4, 2, device="cuda"))
