@@ -453,9 +453,10 @@ Tensor distill_count(const Tensor& like, int64_t vocab, const Tensor& ids, const
   return counts;
 }
 
-// Overwrites the logits [rows, vocab] with their gradient; the loss of each row goes to `loss`.
+// Overwrites the logits [rows, vocab] with their gradient (unless that is not wanted); the loss of each row
+// goes to `loss`.
 void distill_rows_(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const OptTensor& targets, double tau,
-                   double alpha, int64_t ignore_index, const Tensor& counts, const Tensor& loss) {
+                   double alpha, int64_t ignore_index, const Tensor& counts, const Tensor& loss, bool gradient) {
   const c10::cuda::CUDAGuard guard(logits.device());
   auto a = distill_args(logits, logits.size(0), logits.size(1), ids, teacher, targets, {tau, alpha, ignore_index});
   put_logits(a, logits);
@@ -463,7 +464,7 @@ void distill_rows_(const Tensor& logits, const Tensor& ids, const Tensor& teache
               "mmf: distill: counts must be int32 [2]");
   TORCH_CHECK(loss.device() == logits.device() && loss.scalar_type() == torch::kFloat32 && loss.is_contiguous() &&
                   loss.numel() == a.rows, "mmf: distill: loss must be contiguous fp32 [rows]");
-  a.grad = logits.data_ptr();
+  a.grad = gradient ? logits.data_ptr() : nullptr;
   a.grad_ld = a.ld;
   a.counts = counts.data_ptr<int>();
   a.loss = loss.data_ptr<float>();
@@ -618,7 +619,9 @@ void register_lm_ops(pybind11::module_& m) {
   m.def("block_norm", &block_norm);
   m.def("distill", &distill);
   m.def("distill_count", &distill_count);
-  m.def("distill_rows_", &distill_rows_);
+  m.def("distill_rows_", &distill_rows_, py::arg("logits"), py::arg("ids"), py::arg("teacher"), py::arg("targets"),
+        py::arg("tau"), py::arg("alpha"), py::arg("ignore_index"), py::arg("counts"), py::arg("loss"),
+        py::arg("gradient") = true);
   m.def("distill_sum", &distill_sum);
   m.def("distill_scale_", &distill_scale_);
 }

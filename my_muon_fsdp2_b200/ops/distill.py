@@ -139,10 +139,11 @@ def _flat(logits, teacher_ids, teacher_logits, targets, temperature, alpha, redu
 class _LinearDistillFn(torch.autograd.Function):
     """The loss of ``x @ weight.T`` with the logits formed chunk by chunk, like the fused cross entropy:
     per chunk the tcgen05 GEMM for the bf16 logits, the kernel that turns them into their gradient in
-    place, and the GEMMs for dX and dW.  The backward only multiplies by the incoming gradient."""
+    place, and the GEMMs for dX and dW, of which those that are wanted.  The backward only multiplies by
+    the incoming gradient."""
 
     @staticmethod
-    def forward(ctx, x, w, ids, teacher, targets, tau, alpha, ignore_index, chunk):
+    def forward(ctx, x, w, ids, teacher, targets, tau, alpha, ignore_index, chunk, want_x, want_w):
         from .linear import EPI_STORE, gemm, mm_dw, mm_fwd
 
         N, D = x.shape
@@ -154,18 +155,20 @@ class _LinearDistillFn(torch.autograd.Function):
         w_dtype, w = w.dtype, F.pad(w, (0, 0, 0, pad)) if pad else w
         counts = E.distill_count(x, V, ids, teacher, targets, ignore_index)
         rows = torch.empty(N, dtype=torch.float32, device=x.device)
-        dx = torch.empty_like(x)
+        dx = torch.empty_like(x) if want_x else None
         single = N <= chunk
-        dw = torch.empty(V + pad, D, dtype=w.dtype, device=x.device) if single else \
+        dw = None if not want_w else torch.empty(V + pad, D, dtype=w.dtype, device=x.device) if single else \
             torch.zeros(V + pad, D, dtype=torch.float32, device=x.device)
         for s in range(0, N, chunk):
             e = min(N, s + chunk)
             xs = x[s:e]
             (logits,) = mm_fwd(xs, [w])
             E.distill_rows_(logits[:, :V], ids[s:e], teacher[s:e], None if targets is None else targets[s:e], tau, alpha,
-                            ignore_index, counts, rows[s:e])
-            gemm([logits], [w], False, True, [dx[s:e]], EPI_STORE)
-            mm_dw([logits], xs, [dw], accumulate=s > 0)
+                            ignore_index, counts, rows[s:e], want_x or want_w)
+            if want_x:
+                gemm([logits], [w], False, True, [dx[s:e]], EPI_STORE)
+            if want_w:
+                mm_dw([logits], xs, [dw], accumulate=s > 0)
         ctx.kept = (dx, dw)
         ctx.vocab, ctx.w_dtype = V, w_dtype
         return E.distill_sum(rows)
@@ -179,9 +182,10 @@ class _LinearDistillFn(torch.autograd.Function):
         dx, dw = ctx.kept
         ctx.kept = None
         s = g.float().reshape(1)
-        ext().distill_scale_(dx, s)
-        ext().distill_scale_(dw, s)
-        return (dx, dw[:ctx.vocab].to(ctx.w_dtype)) + (None,) * 7
+        for d in (dx, dw):
+            if d is not None:
+                ext().distill_scale_(d, s)
+        return (dx, None if dw is None else dw[:ctx.vocab].to(ctx.w_dtype)) + (None,) * 9
 
 
 def fused_linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
@@ -190,7 +194,8 @@ def fused_linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_ids
                               chunk: int = 8192) -> torch.Tensor:
     """The mean ``distillation_loss`` of the logits ``x @ weight.T`` without holding them all: x [..., dim],
     weight [vocab, dim], the rest as there.  bf16 CUDA tensors run this library's GEMMs around the
-    in-place loss kernel, ``chunk`` tokens at a time; others form the logits in one product."""
+    in-place loss kernel, ``chunk`` tokens at a time, and form the gradients that are wanted (none in an
+    evaluation); others form the logits in one product."""
     if chunk < 1:
         raise ValueError(f"distillation: chunk must be at least 1, got {chunk}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.dtype != weight.dtype or x.device != weight.device:
@@ -212,5 +217,7 @@ def fused_linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_ids
     a = teacher_logits.reshape(ids.shape)
     y = None if targets is None else targets.reshape(-1)
     _check(x2.shape[0], x2.device, weight.shape[0], ids, a, y, temperature, alpha)
+    grad = torch.is_grad_enabled()
     return _LinearDistillFn.apply(x2.contiguous(), weight, ids.contiguous(), a.contiguous(),
-                                  None if y is None else y.contiguous(), temperature, alpha, ignore_index, chunk)
+                                  None if y is None else y.contiguous(), temperature, alpha, ignore_index, chunk,
+                                  grad and x2.requires_grad, grad and weight.requires_grad)

@@ -523,3 +523,36 @@ def test_gpu_forward_mode_is_refused():
         _dual_logits(lambda z, ids, a: distillation_loss(z, ids, a, reduction=reduction), "cuda")
     w = torch.ones(24, 16, device="cuda", dtype=torch.bfloat16)
     _dual_logits(lambda x, ids, a: fused_linear_distillation(x.bfloat16(), w, ids, a), "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk", [8192, 40])
+def test_gpu_fused_linear_forms_what_is_wanted(chunk):
+    """An evaluation, a frozen head and frozen inputs: the same loss, the gradients that are wanted with the same
+    bits, and a GEMM launch and the memory of a gradient less for each that is not."""
+    from my_muon_fsdp2_b200._ext import ext
+
+    g = torch.Generator().manual_seed(0)
+    x, w = (torch.randn(*s, generator=g).to("cuda", torch.bfloat16) for s in ((100, 128), (1003, 128)))
+    _, ids, a, y = _inputs(100, 1003, 6, device="cuda")
+    chunks = -(-100 // chunk)
+
+    def run(want_x, want_w, mode=torch.enable_grad):
+        xs, ws = x.clone().requires_grad_(want_x), w.clone().requires_grad_(want_w)
+        with mode():
+            before = ext().launch_count()
+            loss = fused_linear_distillation(xs, ws, ids, a, y, temperature=2.0, alpha=0.5, chunk=chunk)
+            launches = ext().launch_count() - before
+        if loss.requires_grad:
+            loss.backward()
+        return loss.detach(), xs.grad, ws.grad, launches
+
+    loss, dx, dw, most = run(True, True)
+    for want_x, want_w, mode in ((True, False, torch.enable_grad), (False, True, torch.enable_grad), (False, False, torch.enable_grad),
+                                 (True, True, torch.no_grad), (True, True, torch.inference_mode)):
+        got = run(want_x, want_w, mode)
+        assert torch.equal(got[0], loss)
+        formed = 0 if mode is not torch.enable_grad else want_x + want_w
+        assert most - got[3] == (2 - formed) * chunks
+        for want, mine, full in ((want_x, got[1], dx), (want_w, got[2], dw)):
+            assert torch.equal(mine, full) if want and mode is torch.enable_grad else mine is None
