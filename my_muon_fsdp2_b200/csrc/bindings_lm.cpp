@@ -415,12 +415,13 @@ mmf::DistillArgs distill_args(const Tensor& like, int64_t rows, int64_t vocab, c
   a.ids_32 = it == torch::kInt32;
   a.teacher = teacher.data_ptr();
   a.teacher_dtype = dtype_of(teacher, "teacher logits");
-  a.targets = targets.has_value() ? targets->data_ptr<int64_t>() : nullptr;
   a.rows = rows;
   a.vocab = static_cast<int>(vocab);
   a.top = static_cast<int>(ids.size(1));
   a.tau = static_cast<float>(c.tau);
   a.alpha = static_cast<float>(c.alpha);
+  // without a weight of their own the targets are not looked at, so that none is recorded as bad either
+  a.targets = targets.has_value() && a.alpha < 1.f ? targets->data_ptr<int64_t>() : nullptr;
   a.ignore_index = c.ignore_index;
   return a;
 }
@@ -443,11 +444,11 @@ std::pair<Tensor, Tensor> grad_like(const Tensor& logits) {
   return {flat, flat.as_strided({rows, vocab}, {ld_g, 1}, off)};
 }
 
-// int32 [2]: rows with a slot, rows with a target
+// int32 [2]: rows with a slot, rows with a target (where targets have a weight)
 Tensor distill_count(const Tensor& like, int64_t vocab, const Tensor& ids, const Tensor& teacher,
-                     const OptTensor& targets, int64_t ignore_index) {
+                     const OptTensor& targets, int64_t ignore_index, double alpha) {
   const c10::cuda::CUDAGuard guard(like.device());
-  const auto a = distill_args(like, ids.size(0), vocab, ids, teacher, targets, {1.0, 1.0, ignore_index});
+  const auto a = distill_args(like, ids.size(0), vocab, ids, teacher, targets, {1.0, alpha, ignore_index});
   Tensor counts = torch::empty({2}, like.options().dtype(torch::kInt32));
   mmf::distill_count(a, counts.data_ptr<int>(), cur_stream());
   return counts;
@@ -512,7 +513,7 @@ Tensor distill_forward(const Tensor& logits, const Tensor& ids, const Tensor& te
   a.loss = loss.data_ptr<float>();
   Tensor counts;
   if (mean) {
-    counts = distill_count(logits, a.vocab, ids, teacher, targets, c.ignore_index);
+    counts = distill_count(logits, a.vocab, ids, teacher, targets, c.ignore_index, c.alpha);
     a.counts = counts.data_ptr<int>();
     a.behind_count = true;
     if (counts_kept) *counts_kept = counts;
@@ -618,7 +619,8 @@ void register_lm_ops(pybind11::module_& m) {
   m.def("rotary", &rotary);
   m.def("block_norm", &block_norm);
   m.def("distill", &distill);
-  m.def("distill_count", &distill_count);
+  m.def("distill_count", &distill_count, py::arg("like"), py::arg("vocab"), py::arg("ids"), py::arg("teacher"),
+        py::arg("targets"), py::arg("ignore_index"), py::arg("alpha") = 0.0);
   m.def("distill_rows_", &distill_rows_, py::arg("logits"), py::arg("ids"), py::arg("teacher"), py::arg("targets"),
         py::arg("tau"), py::arg("alpha"), py::arg("ignore_index"), py::arg("counts"), py::arg("loss"),
         py::arg("gradient") = true);

@@ -153,7 +153,7 @@ class _LinearDistillFn(torch.autograd.Function):
         # logits (zero) the loss kernel neither reads nor writes
         pad = -V % 8
         w_dtype, w = w.dtype, F.pad(w, (0, 0, 0, pad)) if pad else w
-        counts = E.distill_count(x, V, ids, teacher, targets, ignore_index)
+        counts = E.distill_count(x, V, ids, teacher, targets, ignore_index, alpha)
         rows = torch.empty(N, dtype=torch.float32, device=x.device)
         dx = torch.empty_like(x) if want_x else None
         single = N <= chunk

@@ -556,3 +556,27 @@ def test_gpu_fused_linear_forms_what_is_wanted(chunk):
         assert most - got[3] == (2 - formed) * chunks
         for want, mine, full in ((want_x, got[1], dx), (want_w, got[2], dw)):
             assert torch.equal(mine, full) if want and mode is torch.enable_grad else mine is None
+
+
+def _targets_without_weight(device):
+    """alpha 1 gives targets no weight: what they hold (another padding than ignore_index, say) does not matter."""
+    z, ids, a, y = _inputs(6, 96, 3, torch.float32, device)
+    bad = torch.where(torch.arange(6, device=device) % 2 == 0, -1, 96)
+    for reduction in ("mean", "none"):
+        want = distillation_loss(z, ids, a, reduction=reduction)
+        assert torch.equal(distillation_loss(z, ids, a, bad, reduction=reduction), want)
+    x, w = torch.ones(6, 16, device=device, dtype=torch.bfloat16), torch.ones(96, 16, device=device, dtype=torch.bfloat16)
+    assert torch.equal(fused_linear_distillation(x, w, ids, a, bad), fused_linear_distillation(x, w, ids, a))
+
+
+def test_targets_without_weight_on_cpu():
+    _targets_without_weight("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_targets_without_weight():
+    from my_muon_fsdp2_b200._ext import check_device_error
+
+    check_device_error(0)
+    _targets_without_weight("cuda")
+    check_device_error(0)  # nothing was recorded
