@@ -115,6 +115,10 @@ class RotaryEmbedding:
         m = s.magnitude if s.magnitude is not None else (0.1 * math.log(s.factor) + 1.0 if s.factor > 1 else 1.0)
         return [r * f / s.factor + (1.0 - r) * f for f, r in zip(base, ramp)], m
 
+    def __getstate__(self):
+        # a saved or copied plan lays its tables out anew: loaded onto another device they would be on the wrong one
+        return {**self.__dict__, "_on": {}}
+
     def to(self, device) -> "RotaryEmbedding":
         self._table(torch.device(device))
         return self

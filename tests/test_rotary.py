@@ -432,3 +432,30 @@ def test_gpu_refused_in_place_call_leaves_versions():
     torch.autograd.grad(out, w)
     apply_rotary(q, k, rot, inplace=True)
     assert q._version == 1 and k._version == 1
+
+
+def test_saved_plan_leaves_its_tables():
+    """Tables of devices stay behind, whatever device the plan is loaded for."""
+    import copy
+    import io
+
+    rot = RotaryEmbedding(8, interleaved=True)
+    rot._on[torch.device("cuda", 0)] = torch.zeros(4, dtype=torch.int64)
+    buf = io.BytesIO()
+    torch.save(rot, buf)
+    buf.seek(0)
+    for other in (torch.load(buf, map_location="cpu", weights_only=False), copy.deepcopy(rot)):
+        assert not other._on and torch.equal(other._turns, rot._turns) and other.interleaved
+    assert rot._on
+
+
+@pytest.mark.gpu
+def test_gpu_saved_plan_on_another_device():
+    import io
+
+    x = _rand((1, 2, 3, 8), torch.float32, "cuda")
+    rot = RotaryEmbedding(8)
+    want, buf = apply_rotary(x, None, rot), io.BytesIO()
+    torch.save(rot, buf)
+    buf.seek(0)
+    assert torch.equal(apply_rotary(x, None, torch.load(buf, map_location="cpu", weights_only=False)), want)
