@@ -416,3 +416,29 @@ def test_forward_mode_is_refused_by_the_entry():
 @pytest.mark.gpu
 def test_gpu_forward_mode_is_refused():
     _duals(lambda t: gated_residual_norm(**t, norm="layer"), SHAPES, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("layer", [False, True], ids=["rms", "layer"])
+@pytest.mark.parametrize("D", [5122, 6001, 8191])
+def test_gpu_rows_over_two_blocks_in_many_turns(D, layer, dtype):
+    """Two blocks a row (widths above 5120; up to there it is four), unequal shares and narrow accesses: more
+    rows than go over the device at once, so that the exchange's places and phases go round."""
+    for n, (gate, lead) in enumerate([("channel", (2, 301)), ("token", (601,)), ("sequence", (3, 211)), ("sequence", (300, 2)), (None, (500,))]):
+        _compare(_inputs(lead, D, dtype, layer, gate, True, True, "cuda", seed=n), layer)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layer", [False, True], ids=["rms", "layer"])
+@pytest.mark.parametrize("D", [64, 1000, 4096, 5000, 8192])
+def test_gpu_backward_of_rows_beside_bad_ones(D, layer):
+    """Infinities and NaN in a row or its gradients stay in that row's dx and dy."""
+    t = _inputs((601,), D, torch.bfloat16, layer, "channel", True, True, "cuda")
+    clean = _run(t, layer, 1e-5, 1.0, 1.0)
+    t["y"][3, 5], t["x"][4, 0], t["dn"][6, 1], t["dh"][300, 2] = float("inf"), float("nan"), float("nan"), float("inf")
+    got = _run(t, layer, 1e-5, 1.0, 1.0)
+    keep = [i for i in range(601) if i not in (3, 4, 6, 300)]
+    for k in ("h", "n", "dx", "dy"):
+        assert torch.equal(got[k][keep], clean[k][keep]), k
+    assert not any(torch.isfinite(got["dx"][i]).all() for i in (3, 4, 6, 300))

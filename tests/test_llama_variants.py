@@ -265,3 +265,30 @@ def test_gpu_wrappers_without_memory_are_refused():
                           fused_linear_distillation)
     with pytest.raises(RuntimeError, match="memory of their own"):
         fused_linear_distillation(x, w, torch.zeros(4, 2, dtype=torch.long, device="cuda"), torch.zeros(4, 2, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_gpu_trainer_distils():
+    """A Trainer's step from host batches: the loss and the gradients of its micro-batches, taken one by one."""
+    from my_muon_fsdp2_b200.train import Trainer
+
+    model, batch = _student(torch.bfloat16, "cuda"), _batch("cpu")
+    tokens = torch.cat([batch[0], batch[1].clamp_min(0)[:, -1:]], 1)
+    host = torch.stack([tokens, tokens.flip(0)])
+    teacher = (torch.stack([batch[3], batch[3].flip(0)]), torch.stack([batch[4], batch[4].flip(0).half().float()]))
+    want, grads = 0.0, [torch.zeros_like(p, dtype=torch.float64) for p in model.parameters()]
+    for i in range(2):
+        t = host[i].cuda()
+        loss = model(t[:, :-1], t[:, 1:], teacher=tuple(x[i].cuda() for x in teacher), temperature=2.0, alpha=0.5)
+        want += loss.item() / 2
+        for s, g in zip(grads, torch.autograd.grad(loss, list(model.parameters()))):
+            s += g.double() / 2
+    tr = Trainer(model, [torch.optim.SGD(model.parameters(), lr=0.0)], grad_accum=2, temperature=2.0, alpha=0.5)
+    kept = {}
+    for n, p in model.named_parameters():
+        p.register_post_accumulate_grad_hook(lambda p, n=n: kept.__setitem__(n, p.grad.clone()))
+    got = tr.train_step(host, teacher)
+    assert abs(got - want) < 1e-5 * abs(want)  # the sum of two fp32 losses
+    for (n, p), g in zip(model.named_parameters(), grads):
+        # halving is exact; the sum of two bf16 gradients is rounded once more
+        assert (kept[n].double() - g).norm() <= 2**-8 * g.norm(), n
