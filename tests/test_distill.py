@@ -580,3 +580,14 @@ def test_gpu_targets_without_weight():
     check_device_error(0)
     _targets_without_weight("cuda")
     check_device_error(0)  # nothing was recorded
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 819200), (torch.float16, 819193), (torch.float32, 409600)], ids=["bf16", "fp16", "fp32"])
+def test_gpu_largest_vocabulary(dtype, V):
+    """The largest rows with the most slots: eight blocks a row, each with all the shared memory that there is."""
+    for n, (tau, reduction) in enumerate([(2.0, "mean"), (1.5, "none")]):
+        _check(*_inputs(3, V, 1024, dtype, "cuda", seed=n), tau, 0.5, reduction, 1024.0 if dtype == torch.float16 else 1.0)
+    z, ids, a, y = _inputs(1, V, 2, dtype, "cuda")
+    with pytest.raises(RuntimeError, match="vocabulary"):
+        distillation_loss(torch.cat([z, z], 1), ids, a, y, alpha=0.5)
