@@ -22,10 +22,12 @@
 // where one block with 16 columns a thread had no registers left for the weights, 330 (303).  Narrower rows
 // are not: at 4096 columns two blocks took 126 us, the exchange being slower than one block's barrier.  A
 // second kernel adds the partials in a fixed order, so that equal calls give equal bits.  8192 x 4096 bf16
-// with both norms and a gate: 92 us, and 5.5 for the sums (403 MB, 67 % of the copy rate); the
-// arithmetic, through packed fp32 instructions, takes about as long as the copies.  With one row a turn 5 us
-// more; unpacked arithmetic, sums in shared memory and no copies ahead 152; 16 columns a thread and two
-// blocks an SM, weights loaded again for each row, 140.
+// with both norms and a gate: 93 us (403 MB, 66 % of the copy rate), and 5.5 for the sums.  One block fills an
+// SM's registers (128 a thread); its warps issue in 57 % of the cycles, the fp32 pipe is 29 % busy, and what
+// they wait for is mostly their own arithmetic and shared memory, two reductions a turn with little else to
+// do beside them.  Layer norms, one row a turn, 143 us; fp32 146, layer 162.  With one row a turn 5 us more;
+// unpacked arithmetic, sums in shared memory and no copies ahead 152; 16 columns a thread and two blocks an SM,
+// weights loaded again for each row, 140.
 #include <algorithm>
 #include <stdexcept>
 #include <string>

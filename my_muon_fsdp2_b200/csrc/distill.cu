@@ -9,17 +9,17 @@
 // KB, one block's shared memory 227): one asynchronous copy in, the maximum and the sums over the
 // slice, one exchange of (maximum, sums) between the blocks, and the gradient straight out of the
 // slice.  Slices of about 32 KB and 256 threads let six blocks share an SM and overlap one another's
-// copies, exchanges and stores; what bounds it is how long a row stays in its block, not the arithmetic
-// (with the exponentials left out it is as slow).  Measured, 4096 x 128256 bf16, 64 slots, tau 2 with hard
-// targets: 405 us (2.1 GB, 79 % of the copy rate), with 8 slots 396, with 256 494 (their rewrites go to as
-// many sectors of their own); slices of 64 KB 445 us; the exchange by a barrier of
-// the cluster, whose release waits for every store before it, and five blocks an SM 510 us; blocks that
-// stay for many rows, two an SM, with copies ahead and the exponentials kept in registers between the
-// two passes 500 us.
+// copies, exchanges and stores.  Measured, 4096 x 128256 bf16, 64 slots, tau 2 with hard targets: 426 us (2.1
+// GB, 75 % of the copy rate), with 8 slots 416, with 256 513 (their rewrites go to as many sectors of their own).
+// The SMs issue in 81 % of the cycles and their pipe for exponentials is 63 % busy: the arithmetic takes nearly
+// as long as the copies, and one exponential less or more a value shows (tau 1 397 us, tau 1.5 594).  Tried at
+// a time when it took 405 us: slices of 64 KB 445; the exchange by a barrier of the cluster, whose release
+// waits for every store before it, and five blocks an SM 510; blocks that stay for many rows, two an SM, with
+// copies ahead and the exponentials kept in registers between the two passes 500.
 //
 // The arithmetic goes through packed fp32 instructions, the maximum of 16-bit types is taken without
 // widening them, and at tau = 2 the softmax at 1 comes from the one at tau as its square (one
-// exponential a value instead of two: 236 instead of 320 us at 2048 rows).
+// exponential a value instead of two).
 //
 // Every exponential is 2^(c (z - m)), m the largest logit of a thread, later of the row.  The difference comes
 // first: it is exactly 0 at the maximum, however far that is from 0 (a row whose words are all at the type's

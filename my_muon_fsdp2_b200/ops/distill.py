@@ -193,9 +193,9 @@ def fused_linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_ids
                               temperature: float = 1.0, alpha: float = 1.0, ignore_index: int = -100,
                               chunk: int = 8192) -> torch.Tensor:
     """The mean ``distillation_loss`` of the logits ``x @ weight.T`` without holding them all: x [..., dim],
-    weight [vocab, dim], the rest as there.  bf16 CUDA tensors run this library's GEMMs around the
-    in-place loss kernel, ``chunk`` tokens at a time, and form the gradients that are wanted (none in an
-    evaluation); others form the logits in one product."""
+    weight [vocab, dim], the rest as there.  bf16 CUDA tensors (dim a multiple of 8, a contiguous weight) run this
+    library's GEMMs around the in-place loss kernel, ``chunk`` tokens at a time, and form the gradients that are
+    wanted (none in an evaluation); others form the logits in one product."""
     if chunk < 1:
         raise ValueError(f"distillation: chunk must be at least 1, got {chunk}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.dtype != weight.dtype or x.device != weight.device:
