@@ -555,7 +555,7 @@ class DistillFn : public torch::autograd::Function<DistillFn> {
     variable_list out(8);
     Tensor up = g[0].to(torch::kFloat32).contiguous();
     const c10::cuda::CUDAGuard guard(up.device());
-    if (ctx->get_saved_variables().empty()) {
+    if (!d.count("tau")) {  // formed in the forward
       TORCH_CHECK(d.count("grad"), "mmf: distill: this loss keeps its gradient for one backward pass; its graph cannot "
                                    "be gone through a second time");
       distill_scale_(d["flat"].toTensor(), up);
@@ -563,7 +563,7 @@ class DistillFn : public torch::autograd::Function<DistillFn> {
       d.clear();
       return out;
     }
-    const auto s = ctx->get_saved_variables();
+    const auto s = ctx->get_saved_variables();  // taken once: a checkpoint hands each out a single time
     const Tensor& logits = s[0];
     const bool mean = d["mean"].toBool();
     const OptTensor targets = s[3].defined() ? OptTensor(s[3]) : OptTensor();

@@ -292,3 +292,37 @@ def test_gpu_trainer_distils():
     for (n, p), g in zip(model.named_parameters(), grads):
         # halving is exact; the sum of two bf16 gradients is rounded once more
         assert (kept[n].double() - g).norm() <= 2**-8 * g.norm(), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [True, False], ids=["reentrant", "not_reentrant"])
+def test_gpu_operators_in_a_checkpoint(reentrant):
+    """Activations formed again in the backward, or kept on the host: the gradients of the plain call, bit by bit."""
+    from torch.utils.checkpoint import checkpoint
+
+    from my_muon_fsdp2_b200.ops.block_norm import gated_residual_norm
+    from my_muon_fsdp2_b200.ops.distill import distillation_loss, fused_linear_distillation
+    from my_muon_fsdp2_b200.ops.rotary import RotaryEmbedding, apply_rotary
+
+    g = torch.Generator().manual_seed(0)
+    rot = RotaryEmbedding(16)
+    pos = torch.arange(6, device="cuda") + 3
+    ids, a = torch.randint(0, 64, (4, 6, 3), generator=g).cuda(), torch.randn(4, 6, 3, generator=g).cuda()
+    y = torch.randint(0, 64, (4, 6), generator=g).cuda()
+    leaves = [torch.randn(s, generator=g).to("cuda", torch.bfloat16).requires_grad_() for s in ((4, 6, 16), (4, 6, 16), (16,), (64, 16))]
+
+    def student(x, z, w, head):
+        h, n = gated_residual_norm(x, z, w, gate=w, pre_weight=w)
+        q = apply_rotary(n.view(4, 6, 1, 16), None, rot, pos).view(4, 6, 16) + h
+        logits = q @ head.t()
+        kd = dict(targets=y, temperature=2.0, alpha=0.5)
+        return fused_linear_distillation(q, head, ids, a, **kd) + distillation_loss(logits, ids, a, **kd) \
+            + distillation_loss(logits, ids, a, reduction="none", **kd).sum() + distillation_loss(logits.half(), ids, a, **kd)
+
+    want = torch.autograd.grad(student(*leaves), leaves)
+    got = [t.detach().clone().requires_grad_() for t in leaves]
+    checkpoint(student, *got, use_reentrant=reentrant).backward()
+    assert all(torch.equal(t.grad, w) for t, w in zip(got, want))
+    with torch.autograd.graph.save_on_cpu():
+        loss = student(*leaves)
+    assert all(torch.equal(t, w) for t, w in zip(torch.autograd.grad(loss, leaves), want))
