@@ -18,7 +18,8 @@
 // and walks over about ten heads, so that sincos is paid once for all heads.  Two heads in flight a
 // thread and four blocks an SM: 8192 tokens x 40 heads x 128 bf16 take 31.6 us (81 % of the copy rate;
 // with four heads in flight and two blocks an SM 43.7), 32768 x 20 x 128 fp32 105 us (97 %).  Where part of
-// the head passes through, the threads that copy it have one load in flight: 3069 tokens x 40 heads x 64 fp16, half rotated, 12.3 us (39 %).
+// the head passes through, the threads that copy it have one load in flight: 3069 tokens x 40 heads x 64
+// fp16, half rotated, 12.3 us (39 %).
 #include <stdexcept>
 #include <string>
 
